@@ -87,6 +87,154 @@ class TargetHead:
         return torch.nn.functional.linear(hidden.to(torch.bfloat16), self.weight)
 
 
+class LogitControls:
+    """Sampling rules of a batch's requests: penalties for tokens that occur in
+    their text, biases, and masks of allowed tokens, applied to the head's
+    logits before a law is taken from them.
+
+        controls = LogitControls(device, vocab, repetition=[1.1, 1.0], presence=[0.0, 0.4],
+                                 frequency=[0.0, 0.2], bias=[None, {42: -3.0}])
+        logits = controls(head(hidden), history, lengths=[812, 90], prompt_lengths=[700, 90],
+                          counts=[7, 7], tokens=tokens, allowed=masks)
+        verify_proposals(logits, tokens, ...)
+
+    Row j of a request is ruled by its history and its first j proposed tokens
+    (which count as answer): a value whose token occurs there is divided by
+    `repetition` if positive and multiplied by it otherwise, then loses
+    `frequency` for each occurrence behind the prompt and `presence` if there is any, then gains
+    its bias; a token that the row's mask does not allow gets `masked`.
+
+    One number or a sequence of one per request (`requests` of them where no sequence says
+    how many); `bias` is None or a {token: bias} mapping (or None) per request.  masked: the value of tokens that are not allowed; None, the
+    lowest finite value of the output's type, gives them no probability in
+    verify_proposals and logits_to_probabilities, which refuse infinite logits;
+    float('-inf') is for samplers that expect it.  A row whose mask allows nothing is -inf
+    throughout, so those two refuse it.  The rules are uploaded once, here."""
+
+    def __init__(self, device, vocab, *, repetition=1.0, presence=0.0, frequency=0.0, bias=None, masked=None,
+                 requests=None):
+        if type(vocab) is not int or not 1 <= vocab < 2 ** 31:
+            raise ValueError('vocab must be a positive integer')
+        per_request = [x for x in (repetition, presence, frequency, bias) if x is not None and not isinstance(x, Real)]
+        lengths = {len(x) for x in per_request}
+        if requests is not None:
+            lengths.add(requests)
+        n = lengths.pop() if lengths else 1
+        if lengths or type(n) is not int or not 1 <= n <= 65535:
+            raise ValueError('Penalties and biases must name the same number of requests, 1 to 65535')
+        self.requests, self.vocab = n, vocab
+        rules = []
+        for name, x in (('repetition', repetition), ('presence', presence), ('frequency', frequency)):
+            x = [x] * n if isinstance(x, Real) else list(x)
+            if any(isinstance(p, bool) or not isinstance(p, Real) or not abs(p) <= torch.finfo(torch.float32).max
+                   for p in x):
+                raise ValueError(f'{name} must be finite')
+            if name == 'repetition' and min(x) < 2.0 ** -126:
+                raise ValueError('repetition must be positive')
+            rules += [float(p) for p in x]
+        start, tokens, values = [0], [], []
+        for d in [None] * n if bias is None else bias:
+            for token, value in sorted((d or {}).items()):
+                if type(token) is not int or not 0 <= token < vocab:
+                    raise ValueError('Biased tokens must be integers in the vocabulary')
+                if isinstance(value, bool) or not isinstance(value, Real) \
+                        or not abs(value) <= torch.finfo(torch.float32).max:
+                    raise ValueError('Biases must be finite')
+                tokens.append(token)
+                values.append(float(value))
+            start.append(len(tokens))
+        if masked is not None and (isinstance(masked, bool) or not isinstance(masked, Real) or masked != masked):
+            raise ValueError('masked must be a number or None')
+        self.masked = masked
+        self.device = require_gfx950(device)
+        self._penalties = upload(self.device, rules, torch.float64)
+        self._bias_start = upload(self.device, start)
+        self._bias_token = upload(self.device, tokens)
+        self._bias_value = upload(self.device, values, torch.float64)
+        self._stream = torch.cuda.current_stream(self.device)
+        self._uploaded = torch.cuda.Event()
+        self._uploaded.record(self._stream)
+
+    @torch.no_grad()
+    def __call__(self, logits, history, *, lengths, prompt_lengths=None, counts=None, tokens=None, slots=None,
+                 allowed=None, out=None):
+        """logits [rows, vocab] bf16 or fp32, request-major; history: int32 or int64
+        [texts, capacity], of which request r's text is row slots[r] (default: r), its first
+        lengths[r] tokens, prompt_lengths[r] (default: none) of them a prompt.
+        counts: proposed tokens per request (default: none), whose rows number
+        counts[r] + 1; tokens: the proposed tokens, as verify_proposals takes them.
+        allowed: int32 [rows, ceil(vocab / 32)], token v is bit v % 32 of word v // 32.
+        out: a tensor for the result, of the logits' type or fp32 (default: a
+        new one of the logits' type); it may be `logits`, else must not overlap it."""
+        dtype = _logits(logits)
+        if logits.device != self.device or logits.shape[1] != self.vocab:
+            raise ValueError(f'Logits must be [rows, {self.vocab}] on the controls\' device')
+        if torch.cuda.is_current_stream_capturing():
+            raise ValueError('The lengths are uploaded with each call, which a captured graph cannot repeat')
+        lengths = [int(x) for x in lengths]
+        n = len(lengths)
+        prompts = [0] * n if prompt_lengths is None else [int(x) for x in prompt_lengths]
+        counts = [0] * n if counts is None else [int(x) for x in counts]
+        slots = list(range(n)) if slots is None else [int(x) for x in slots]
+        if n != self.requests:
+            raise ValueError(f'These controls rule {self.requests} requests')
+        if not len(prompts) == len(counts) == len(slots) == n:
+            raise ValueError('One length, prompt length, proposal length and text per request required')
+        if any(x < 0 for x in counts) or len(logits) != sum(counts) + n:
+            raise ValueError('Each request has a row for each of its proposed tokens and one more')
+        if max(counts) > MAX_PROPOSAL:
+            raise ValueError(_ERRORS[6])
+        if (not isinstance(history, torch.Tensor) or history.ndim != 2 or history.device != self.device
+                or history.dtype not in (torch.int32, torch.int64) or history.stride(1) != 1 and history.shape[1] > 1):
+            raise ValueError('history must be int32 or int64 [texts, capacity] with contiguous rows')
+        if any(not 0 <= s < len(history) for s in slots) \
+                or any(not 0 <= p <= x <= history.shape[1] for p, x in zip(prompts, lengths)):
+            raise ValueError('Texts must lie within history, prompts within their texts')
+        total = sum(counts)
+        if total and (not isinstance(tokens, torch.Tensor) or tokens.dtype != torch.long or tokens.shape != (total,)
+                      or tokens.device != self.device):
+            raise ValueError('tokens must be the proposed tokens, int64, on the controls\' device')
+        words = (self.vocab + 31) // 32
+        if allowed is not None and (
+                not isinstance(allowed, torch.Tensor) or allowed.dtype != torch.int32 or allowed.device != self.device
+                or allowed.ndim != 2 or allowed.shape[0] != len(logits) or allowed.shape[1] < words
+                or allowed.stride(1) != 1 or allowed.stride(0) < words):
+            raise ValueError('allowed must be int32 [rows, ceil(vocab / 32)] with contiguous rows')
+        if out is None:
+            out = torch.empty(logits.shape, dtype=logits.dtype, device=self.device)
+        elif (not isinstance(out, torch.Tensor) or out.shape != logits.shape or out.device != self.device
+              or out.dtype not in (logits.dtype, torch.float32) or out.stride(1) != 1 or out.stride(0) < self.vocab):
+            raise ValueError('out must be [rows, vocab] of the logits\' type or fp32, with contiguous rows')
+        elif _overlap(out, logits) and (out.data_ptr() != logits.data_ptr() or out.dtype != logits.dtype
+                                        or out.stride() != logits.stride()):
+            raise ValueError('out must be the logits or not overlap them')
+        if logits.stride(0) < self.vocab:
+            raise ValueError('Logit rows must not overlap')
+        stream = torch.cuda.current_stream(self.device)
+        if stream != self._stream:
+            stream.wait_event(self._uploaded)
+        cu = [0]
+        for x in counts:
+            cu.append(cu[-1] + x + 1)
+        head = upload(self.device, cu + slots + lengths + prompts)
+        fill = torch.finfo(out.dtype).min if self.masked is None else self.masked
+        _native.call('dspark_logit_controls', logits.data_ptr(), dtype, logits.stride(0), self.vocab, head.data_ptr(), n,
+                     head[n + 1:].data_ptr(), history.data_ptr() or head.data_ptr(), history.element_size(),
+                     history.stride(0), tokens.contiguous().data_ptr() if total else None, self._penalties.data_ptr(),
+                     self._bias_start.data_ptr(), self._bias_token.data_ptr() or None, self._bias_value.data_ptr() or None,
+                     None if allowed is None else allowed.data_ptr(), 0 if allowed is None else allowed.stride(0), fill,
+                     out.data_ptr(), 0 if out.dtype == torch.bfloat16 else 1, out.stride(0), stream.cuda_stream)
+        return out
+
+
+def _overlap(a, b):
+    """Whether two row-contiguous matrices share memory, by the spans they lie in."""
+    def span(t):
+        return t.data_ptr(), t.data_ptr() + t.element_size() * ((t.shape[0] - 1) * t.stride(0) + t.shape[1])
+    (a0, a1), (b0, b1) = span(a), span(b)
+    return a0 < b1 and b0 < a1
+
+
 _WORKSPACES = {}
 
 
