@@ -16,8 +16,8 @@ LIB_PATH = os.path.join(BUILD_DIR, LIB_NAME)
 # draft kernel (DSPARK_TIMELINE); loaded instead of LIB_PATH only when the
 # DSPARK_AMD_TIMELINE environment variable is set (bench.py --timeline).
 TIMELINE_LIB_PATH = os.path.join(BUILD_DIR, 'libdspark_amd_timeline.so')
-SOURCES = ('attn.hip', 'kv.hip', 'layout.hip', 'prologue.hip', 'project.hip', 'sample.hip', 'controls.hip',
-           'measure.hip', 'errors.cpp')
+SOURCES = ('attn.hip', 'kv.hip', 'layout.hip', 'prologue.hip', 'adapters.hip', 'project.hip', 'sample.hip',
+           'controls.hip', 'measure.hip', 'errors.cpp')
 ARCH = 'gfx950'
 # Packed FP32 VALU ops are disabled for all device code.
 FLAGS = ('--offload-arch=' + ARCH, '-O3', '-std=c++17', '-shared', '-fPIC',

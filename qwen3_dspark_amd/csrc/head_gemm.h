@@ -98,15 +98,16 @@ using HeadLane = HeadLaneOf<2>;
 // rows (row stride `hidden`), `tokens` of them; t0: the workgroup's first
 // token.  Rows past `tokens` re-read the last token (their results are
 // discarded by the caller).  pre_combine() runs once the ring has drained
-// and before the exchange (a place to issue the epilogue's global loads).
+// and before the exchange (a place to issue the epilogue's global loads); extra(acc)
+// before it may add further products to the wave's accumulators (its K half's share).
 // With SUMSQ, ss receives sum(x^2) over the lane's token row (the same
 // value in all lanes of that token).  The exchange is read after the
 // function's last barrier: afterwards the caller may use only the
 // HG_ROW_OFF region (head_row_sumsq) of the ring's LDS.
-template <bool SUMSQ, int TG = 2, typename PreCombine>
+template <bool SUMSQ, int TG = 2, typename PreCombine, typename Extra>
 __device__ __forceinline__ void head_tile_gemm(const bf16* __restrict__ w, const bf16* __restrict__ x, int tokens,
                                                int hidden, int t0, unsigned char* smem, float (&v)[2][8], float& ss,
-                                               PreCombine&& pre_combine) {
+                                               PreCombine&& pre_combine, Extra&& extra) {
   const int lane = threadIdx.x & 63;
   const int wave = threadIdx.x >> 6;
   using Ring = HeadRing<TG>;
@@ -175,6 +176,7 @@ __device__ __forceinline__ void head_tile_gemm(const bf16* __restrict__ w, const
     }
     __builtin_amdgcn_sched_barrier(0);    // the next stage's wait not above these MFMAs
   }
+  extra(acc);
   pre_combine();
   __syncthreads();   // every wave is done with the ring: reuse it for the exchange
 
@@ -207,6 +209,13 @@ __device__ __forceinline__ void head_tile_gemm(const bf16* __restrict__ w, const
       for (int i = 0; i < 4; ++i) v[a][4 * q + i] = (L.kq == 0 ? acc[a][4 * q + i] : acc[a][8 + 4 * q + i]) + o[i];
     }
   if (SUMSQ) ss += ssx[(wave ^ (2 * TG)) * 64 + lane];  // the other column half of the row
+}
+
+template <bool SUMSQ, int TG = 2, typename PreCombine>
+__device__ __forceinline__ void head_tile_gemm(const bf16* __restrict__ w, const bf16* __restrict__ x, int tokens,
+                                               int hidden, int t0, unsigned char* smem, float (&v)[2][8], float& ss,
+                                               PreCombine&& pre_combine) {
+  head_tile_gemm<SUMSQ, TG>(w, x, tokens, hidden, t0, smem, v, ss, pre_combine, [](f32x16 (&)[2]) {});
 }
 
 // sum over the 128 dims of v^2 for the lane's token.  Every wave of the

@@ -20,6 +20,7 @@
 // MFMA tile (head_gemm.h); all its waves run the epilogue on 16 dims of one
 // token per lane.  Accumulation and the epilogue are FP32; outputs are
 // rounded to bf16 once.
+#include "adapters.h"
 #include "wide_gemm.h"
 
 namespace dspark {
@@ -44,9 +45,9 @@ struct PrologueArgs {
 };
 
 // grid: 32 heads (0-15 q, 16-23 k, 24-31 v) x ceil(T / (32 TG)) token tiles, one
-// dimension (see the XCD mapping below); 4 TG waves.
-template <int TG>
-__global__ __launch_bounds__(4 * TG * WAVE) void qkv_prologue_kernel(PrologueArgs a) {
+// dimension (see the XCD mapping below); 4 TG waves.  ADAPT: with low-rank adapters.
+template <int TG, bool ADAPT = false>
+__global__ __launch_bounds__(4 * TG * WAVE) void qkv_prologue_kernel(PrologueArgs a, AdapterArgs ad) {
   __shared__ __attribute__((aligned(16))) unsigned char smem[HeadRing<TG>::SMEM];
   // XCD-aware placement: workgroups are dealt round-robin over the 8 XCDs
   // (each with its own L2), so the token tiles of one head are given ids
@@ -70,13 +71,23 @@ __global__ __launch_bounds__(4 * TG * WAVE) void qkv_prologue_kernel(PrologueArg
   float v[2][8];
   float ss;
   // the epilogue's operands are fetched while the K halves are exchanged
-  head_tile_gemm<false, TG>(w, a.x, a.tokens, a.hidden, t0, smem, v, ss, [&]() {
+  auto fetch = [&]() {
     if (kind < 2) {
       nw.load(kind == 0 ? a.q_norm : a.k_norm);
       if (a.rope) rope.load(a.rope + (size_t)tok * 128);
       else pos = (float)a.positions[tok];
     }
-  });
+  };
+  if constexpr (ADAPT) {
+    head_tile_gemm<false, TG>(w, a.x, a.tokens, a.hidden, t0, smem, v, ss, fetch, [&](f32x16 (&acc)[2]) {
+      const int id[1] = {ad.token[tok]};
+      const bf16* const u[1] = {ad.u + ((size_t)kind * a.tokens + tok) * 2 * ad.rank};
+      adapter_expand<1>([&](int i, int) -> f32x16& { return acc[i]; }, ad, head, id, u,
+                        [&](int i) { return 32 * (L.dh + 2 * i) + L.n; }, L.kq, 2);
+    });
+  } else {
+    head_tile_gemm<false, TG>(w, a.x, a.tokens, a.hidden, t0, smem, v, ss, fetch);
+  }
   if (kind < 2) {
     head_rms_norm(v, nw, a.eps, head_row_sumsq<TG>(v, smem));
     if (!a.rope) rope.compute(a.inv_freq, pos);
@@ -87,8 +98,8 @@ __global__ __launch_bounds__(4 * TG * WAVE) void qkv_prologue_kernel(PrologueArg
 }
 
 // The same for many tokens: 128-token tiles (wide_gemm.h), two workgroups per CU.
-template <bool TABLE>
-__global__ __launch_bounds__(WG_WAVES * WAVE, 2) void qkv_prologue_wide_kernel(PrologueArgs a) {
+template <bool TABLE, bool ADAPT = false>
+__global__ __launch_bounds__(WG_WAVES * WAVE, 2) void qkv_prologue_wide_kernel(PrologueArgs a, AdapterArgs ad) {
   __shared__ __attribute__((aligned(16))) unsigned char smem[WG_SMEM];
   const int tiles = (a.tokens + WG_TOKENS - 1) / WG_TOKENS;
   const int xcd = blockIdx.x & 7;                // a head's tiles share id % 8 (see above)
@@ -101,6 +112,19 @@ __global__ __launch_bounds__(WG_WAVES * WAVE, 2) void qkv_prologue_wide_kernel(P
   f32x16 v[2][2];
   wide_tile_gemm(w, a.x, a.tokens, a.hidden, t0, smem, v);
   const WideLane L;
+  if constexpr (ADAPT) {
+    int id[2];
+    const bf16* u[2];
+    #pragma unroll
+    for (int tt = 0; tt < 2; ++tt) {
+      const int tok = min(t0 + L.token(tt), a.tokens - 1);
+      id[tt] = ad.token[tok];
+      u[tt] = ad.u + ((size_t)kind * a.tokens + tok) * 2 * ad.rank;
+    }
+    const bf16* const uc[2] = {u[0], u[1]};
+    adapter_expand<2>([&](int i, int tt) -> f32x16& { return v[i][tt]; }, ad, head, id, uc,
+                      [&](int i) { return 32 * (L.dh + 2 * i) + L.n; }, 0, 1);
+  }
   if (kind < 2) {
     int tok[2];
     float pos[2];
@@ -165,11 +189,29 @@ constexpr int PROLOGUE_WIDE_TOKENS = 513;
 // 10.4 / 12.1, 224 10.3 / 11.6, 256 10.3 / 11.8.
 constexpr int PROLOGUE_NARROW_TOKENS = 256;
 
-extern "C" int dspark_qkv_prologue(const void* x, const void* wq, const void* wk, const void* wv,
-                                   const void* q_norm, const void* k_norm, const float* inv_freq,
-                                   const int64_t* positions, const float* rope, int tokens, int hidden, float eps,
-                                   void* q_out, void* k_out, void* v_out, int64_t kv_row_stride, void* stream) {
-  clear_error();
+namespace {
+
+template <bool ADAPT>
+int launch_prologue(const PrologueArgs& a, const AdapterArgs& ad, hipStream_t s) {
+  constexpr int HEADS = HQ + 2 * HKV;
+  if (a.tokens >= PROLOGUE_WIDE_TOKENS) {
+    const dim3 grid(HEADS * ((a.tokens + WG_TOKENS - 1) / WG_TOKENS));
+    if (a.rope) hipLaunchKernelGGL((qkv_prologue_wide_kernel<true, ADAPT>), grid, dim3(WG_WAVES * WAVE), 0, s, a, ad);
+    else hipLaunchKernelGGL((qkv_prologue_wide_kernel<false, ADAPT>), grid, dim3(WG_WAVES * WAVE), 0, s, a, ad);
+    return launch_status("qkv_prologue_wide_kernel");
+  }
+  if (a.tokens <= PROLOGUE_NARROW_TOKENS) {
+    hipLaunchKernelGGL((qkv_prologue_kernel<1, ADAPT>), dim3(HEADS * ((a.tokens + 31) / 32)), dim3(4 * WAVE), 0, s, a, ad);
+    return launch_status("qkv_prologue_kernel");
+  }
+  hipLaunchKernelGGL((qkv_prologue_kernel<2, ADAPT>), dim3(HEADS * ((a.tokens + HG_TOKENS - 1) / HG_TOKENS)),
+                     dim3(HG_WAVES * WAVE), 0, s, a, ad);
+  return launch_status("qkv_prologue_kernel");
+}
+
+int check_prologue(PrologueArgs& a, const void* x, const void* wq, const void* wk, const void* wv, const void* q_norm,
+                   const void* k_norm, const float* inv_freq, const int64_t* positions, const float* rope, int tokens,
+                   int hidden, float eps, void* q_out, void* k_out, void* v_out, int64_t kv_row_stride) {
   DSPARK_REQUIRE(x && wq && wk && wv && q_norm && k_norm && inv_freq && positions && q_out && k_out && v_out,
                  "null pointer argument");
   DSPARK_REQUIRE(tokens >= 1 && hidden >= HG_COLS && hidden % HG_COLS == 0, "need tokens >= 1 and hidden a multiple of %d",
@@ -180,25 +222,42 @@ extern "C" int dspark_qkv_prologue(const void* x, const void* wq, const void* wk
                         (uintptr_t)k_out | (uintptr_t)v_out | (uintptr_t)inv_freq | (uintptr_t)rope;
   DSPARK_REQUIRE(any % 16 == 0, "tensors must be 16-byte aligned");
   DSPARK_REQUIRE(((uintptr_t)q_norm | (uintptr_t)k_norm) % 8 == 0, "norm weights must be 8-byte aligned");
-  PrologueArgs a{static_cast<const bf16*>(x), static_cast<const bf16*>(wq), static_cast<const bf16*>(wk),
-                 static_cast<const bf16*>(wv), static_cast<const bf16*>(q_norm), static_cast<const bf16*>(k_norm),
-                 inv_freq, positions, rope, static_cast<bf16*>(q_out), static_cast<bf16*>(k_out),
-                 static_cast<bf16*>(v_out), kv_row_stride, tokens, hidden, eps};
-  if (tokens >= PROLOGUE_WIDE_TOKENS) {
-    const dim3 grid((HQ + 2 * HKV) * ((tokens + WG_TOKENS - 1) / WG_TOKENS));
-    hipStream_t s = static_cast<hipStream_t>(stream);
-    if (rope) hipLaunchKernelGGL(qkv_prologue_wide_kernel<true>, grid, dim3(WG_WAVES * WAVE), 0, s, a);
-    else hipLaunchKernelGGL(qkv_prologue_wide_kernel<false>, grid, dim3(WG_WAVES * WAVE), 0, s, a);
-    return launch_status("qkv_prologue_wide_kernel");
-  }
-  if (tokens <= PROLOGUE_NARROW_TOKENS) {
-    hipLaunchKernelGGL(qkv_prologue_kernel<1>, dim3((HQ + 2 * HKV) * ((tokens + 31) / 32)), dim3(4 * WAVE), 0,
-                       static_cast<hipStream_t>(stream), a);
-    return launch_status("qkv_prologue_kernel");
-  }
-  hipLaunchKernelGGL(qkv_prologue_kernel<2>, dim3((HQ + 2 * HKV) * ((tokens + HG_TOKENS - 1) / HG_TOKENS)),
-                     dim3(HG_WAVES * WAVE), 0, static_cast<hipStream_t>(stream), a);
-  return launch_status("qkv_prologue_kernel");
+  a = PrologueArgs{static_cast<const bf16*>(x), static_cast<const bf16*>(wq), static_cast<const bf16*>(wk),
+                   static_cast<const bf16*>(wv), static_cast<const bf16*>(q_norm), static_cast<const bf16*>(k_norm),
+                   inv_freq, positions, rope, static_cast<bf16*>(q_out), static_cast<bf16*>(k_out),
+                   static_cast<bf16*>(v_out), kv_row_stride, tokens, hidden, eps};
+  return OK;
+}
+
+}  // namespace
+
+extern "C" int dspark_qkv_prologue(const void* x, const void* wq, const void* wk, const void* wv,
+                                   const void* q_norm, const void* k_norm, const float* inv_freq,
+                                   const int64_t* positions, const float* rope, int tokens, int hidden, float eps,
+                                   void* q_out, void* k_out, void* v_out, int64_t kv_row_stride, void* stream) {
+  clear_error();
+  PrologueArgs a{};
+  const int rc = check_prologue(a, x, wq, wk, wv, q_norm, k_norm, inv_freq, positions, rope, tokens, hidden, eps, q_out,
+                                k_out, v_out, kv_row_stride);
+  return rc != OK ? rc : launch_prologue<false>(a, AdapterArgs{}, static_cast<hipStream_t>(stream));
+}
+
+extern "C" int dspark_qkv_prologue_adapted(const void* x, const void* wq, const void* wk, const void* wv,
+                                           const void* q_norm, const void* k_norm, const float* inv_freq,
+                                           const int64_t* positions, const float* rope, int tokens, int hidden,
+                                           float eps, const int32_t* token_adapter, const void* b, int adapters,
+                                           int rank, const void* u, void* q_out, void* k_out, void* v_out,
+                                           int64_t kv_row_stride, void* stream) {
+  clear_error();
+  DSPARK_REQUIRE(token_adapter && b && u, "null pointer argument");
+  DSPARK_REQUIRE(adapters >= 1 && rank >= 16 && rank % 16 == 0 && rank <= 256,
+                 "need adapters >= 1 and rank a multiple of 16 up to 256");
+  DSPARK_REQUIRE((((uintptr_t)b | (uintptr_t)u) & 15) == 0, "tensors must be 16-byte aligned");
+  PrologueArgs a{};
+  const int rc = check_prologue(a, x, wq, wk, wv, q_norm, k_norm, inv_freq, positions, rope, tokens, hidden, eps, q_out,
+                                k_out, v_out, kv_row_stride);
+  const AdapterArgs ad{token_adapter, static_cast<const bf16*>(b), static_cast<const bf16*>(u), adapters, rank};
+  return rc != OK ? rc : launch_prologue<true>(a, ad, static_cast<hipStream_t>(stream));
 }
 
 extern "C" int dspark_rope_table(const float* inv_freq, const int64_t* positions, int tokens, float* table,

@@ -610,12 +610,13 @@ class PersistentTargetKV:
         self._staged.add(layer)
 
     @torch.no_grad()
-    def stage_projected(self, tx, layer, hidden, prologue):
+    def stage_projected(self, tx, layer, hidden, prologue, *, adapters=None, batch=None):
         """Run the layer's attention prologue (QKVPrologue: q/k/v projection,
         q/k RMSNorm, RoPE at each row's absolute position) on the packed
         hidden states [sum Q, H] and write K/V straight into this layer's
         scratch - stage_layer without the separate copy.  Returns the
-        queries [sum Q, 16, 128] for attend()."""
+        queries [sum Q, 16, 128] for attend().  adapters, batch: the layer's low-rank
+        adapters and which of them each request has (QKVPrologue.__call__)."""
         ws = self._of(tx)
         self._stage_target(layer)
         self._check_fused_storage('The fused prologue')
@@ -624,8 +625,9 @@ class PersistentTargetKV:
         rope = self._rope.get(prologue.theta)
         if rope is None:                 # once per transaction: every layer's rows sit at the same positions
             rope = self._rope[prologue.theta] = prologue.rope_table(ws.positions)
+        given = {} if adapters is None and batch is None else dict(adapters=adapters, batch=batch)
         queries, _, _ = prologue(hidden, ws.positions, k_out=self.scratch_keys[layer], v_out=self.scratch_values[layer],
-                                 rope=rope)
+                                 rope=rope, **given)
         self._staged.add(layer)
         return queries
 

@@ -78,11 +78,13 @@ class QKVPrologue:
                      _native.stream_handle(self.device))
         return table
 
-    def __call__(self, hidden, positions, *, k_out=None, v_out=None, rope=None):
+    def __call__(self, hidden, positions, *, k_out=None, v_out=None, rope=None, adapters=None, batch=None):
         """hidden [T, H] bf16, positions [T] int64 (device) -> (q [T,16,128],
         k, v [T,8,128]).  k_out/v_out: optional destinations whose token rows
         are 8*128 elements apart (e.g. a scratch layer); they are returned.
-        rope: optional rope_table(positions) of a prologue with this theta."""
+        rope: optional rope_table(positions) of a prologue with this theta.
+        adapters, batch: this layer's low-rank adapters (adapters.QKVAdapters) and which
+        of them each request of the batch has (adapters.AdapterBatch)."""
         t = hidden.shape[0] if isinstance(hidden, torch.Tensor) and hidden.ndim == 2 else 0
         if (t < 1 or hidden.shape[1] != self.hidden or hidden.dtype != torch.bfloat16
                 or hidden.device != self.device or not hidden.is_contiguous()):
@@ -92,6 +94,10 @@ class QKVPrologue:
                                  or tuple(rope.shape) != (t, HEAD_DIM) or rope.device != self.device
                                  or not rope.is_contiguous()):
             raise ValueError('Rotary table must be a contiguous float32 [T, 128] device tensor (rope_table)')
+        if (adapters is None) != (batch is None):
+            raise ValueError('adapters and batch go together')
+        if adapters is not None:
+            adapters.check(batch, t, self.hidden, self.device)
         q = torch.empty((t, Q_HEADS, HEAD_DIM), dtype=torch.bfloat16, device=self.device)
         outs = []
         for o in (k_out, v_out):
@@ -103,8 +109,15 @@ class QKVPrologue:
                 raise ValueError('K/V destinations must be bf16 [>=T, 8, 128] token-major on the device')
             outs.append(o)
         wq, wk, wv, qn, kn = self.weights
-        _native.call('dspark_qkv_prologue', hidden.data_ptr(), wq.data_ptr(), wk.data_ptr(), wv.data_ptr(),
-                     qn.data_ptr(), kn.data_ptr(), self.inv_freq.data_ptr(), positions.data_ptr(),
-                     rope.data_ptr() if rope is not None else None, t, self.hidden, self.eps, q.data_ptr(),
-                     outs[0].data_ptr(), outs[1].data_ptr(), KV_HEADS * HEAD_DIM, _native.stream_handle(self.device))
+        given = (hidden.data_ptr(), wq.data_ptr(), wk.data_ptr(), wv.data_ptr(), qn.data_ptr(), kn.data_ptr(),
+                 self.inv_freq.data_ptr(), positions.data_ptr(), rope.data_ptr() if rope is not None else None, t,
+                 self.hidden, self.eps)
+        into = (q.data_ptr(), outs[0].data_ptr(), outs[1].data_ptr(), KV_HEADS * HEAD_DIM,
+                _native.stream_handle(self.device))
+        if adapters is not None and batch.n_tiles:
+            u = adapters.shrink(hidden, batch)
+            _native.call('dspark_qkv_prologue_adapted', *given, batch.token_adapter.data_ptr(), adapters.b.data_ptr(),
+                         adapters.count, adapters.padded_rank, u.data_ptr(), *into)
+        else:
+            _native.call('dspark_qkv_prologue', *given, *into)
         return q, outs[0], outs[1]

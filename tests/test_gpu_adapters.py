@@ -1,0 +1,201 @@
+"""Low-rank adapters beside the q/k/v projection, against the formula in float64, over
+the prologue's three tilings (up to 256, 512 and more tokens)."""
+import pytest
+import torch
+
+from helpers import SEED
+
+pytestmark = pytest.mark.gpu
+DEV = torch.device('cuda:0')
+H, D, EPS = 1024, 128, 1e-6
+HEADS = dict(q=16, k=8, v=8)
+
+
+def rnd(gen, *shape, scale=1.0):
+    return (scale * torch.randn(*shape, generator=gen)).to(torch.bfloat16).to(DEV)
+
+
+class Layer:
+    def __init__(self, adapters, rank, hidden=H, seed=0):
+        from qwen3_dspark_amd.adapters import QKVAdapters
+        from qwen3_dspark_amd.prologue import QKVPrologue
+        gen = torch.Generator().manual_seed(SEED + seed)
+        s = hidden ** -0.5
+        self.hidden, self.gen = hidden, gen
+        self.w = {p: rnd(gen, h * D, hidden, scale=s) for p, h in HEADS.items()}
+        self.norm = {p: 1 + rnd(gen, D, scale=0.2) for p in 'qk'}
+        self.a = {p: rnd(gen, adapters, rank, hidden, scale=s) for p in 'qkv'}
+        self.b = {p: rnd(gen, adapters, h * D, rank, scale=rank ** -0.5) for p, h in HEADS.items()}
+        self.scaling = [0.25 + 0.5 * (i % 3) for i in range(adapters)]
+        self.prologue = QKVPrologue(self.w['q'], self.w['k'], self.w['v'], self.norm['q'], self.norm['k'], eps=EPS)
+        self.adapters = QKVAdapters(*(x for p in 'qkv' for x in (self.a[p], self.b[p])), scaling=self.scaling)
+
+    def inputs(self, tokens):
+        x = rnd(self.gen, tokens, self.hidden)
+        positions = torch.randint(0, 9000, (tokens,), generator=self.gen).to(DEV)
+        return x, positions, self.prologue.rope_table(positions)
+
+    def expected(self, x, rope, lengths, ids):
+        outs = []
+        for p, h in HEADS.items():
+            y = x.double() @ self.w[p].double().T.contiguous()
+            at = 0
+            for n, a in zip(lengths, ids):
+                if a >= 0:
+                    low = x[at:at + n].double() @ self.a[p][a].double().T.contiguous()
+                    y[at:at + n] += self.scaling[a] * (low @ self.b[p][a].double().T.contiguous())
+                at += n
+            y = y.view(-1, h, D)
+            if p != 'v':
+                y = y * torch.rsqrt(y.square().mean(-1, keepdim=True) + EPS) * self.norm[p].double()
+                c, s = rope.double()[:, None, :64], rope.double()[:, None, 64:]
+                y = torch.cat((y[..., :64] * c - y[..., 64:] * s, y[..., 64:] * c + y[..., :64] * s), -1)
+            outs.append(y)
+        return outs
+
+
+def check(got, want):
+    """The output's rounding (2^-8), and sums of 1,024 products in FP32: 1,024 2^-24 times
+    the sum of their magnitudes, about 20 for weights of deviation 1/32, is 1.2e-3 against a head's
+    largest value of 3 and more."""
+    for g, w in zip(got, want):
+        assert torch.isfinite(g).all()
+        off = (g.double() - w).abs() - 2 ** -8 * w.abs()
+        assert (off <= 4e-4 * w.abs().amax(-1, keepdim=True)).all(), float(off.max())
+
+
+@pytest.mark.parametrize('lengths,ids', [
+    ([1], [0]), ([1, 1, 1], [2, -1, 2]), ([7] * 9, [0, 1, 2, 2, 1, 0, -1, 2, 1]), ([31, 2], [1, 1]), ([33], [2]),
+    ([5, 60, 1, 200], [0, -1, 1, 2]), ([1] * 300, [i % 4 - 1 for i in range(300)]), ([130, 383], [2, 1]),
+    ([7] * 80, [i % 3 for i in range(80)]), ([900, 3, 250, 1], [-1, 0, 1, 2])])
+@pytest.mark.parametrize('rank', [1, 16, 40])
+def test_against_the_formula(lengths, ids, rank):
+    from qwen3_dspark_amd.adapters import AdapterBatch
+    layer = Layer(3, rank, seed=rank)
+    x, positions, rope = layer.inputs(sum(lengths))
+    batch = AdapterBatch(DEV, lengths, ids)
+    got = layer.prologue(x, positions, rope=rope, adapters=layer.adapters, batch=batch)
+    check(got, layer.expected(x, rope, lengths, ids))
+    again = layer.prologue(x, positions, adapters=layer.adapters, batch=batch)      # angles formed in the kernel
+    assert all(torch.equal(a, b) for a, b in zip(got, again))
+    plain = layer.prologue(x, positions, rope=rope)
+    bare = torch.tensor([a < 0 for n, a in zip(lengths, ids) for _ in range(n)], device=DEV)
+    assert all(torch.equal(a[bare], b[bare]) for a, b in zip(got, plain))
+
+
+@pytest.mark.parametrize('hidden,rank,adapters', [(128, 256, 2), (256, 3, 1), (2048, 64, 5)])
+def test_sizes(hidden, rank, adapters):
+    from qwen3_dspark_amd.adapters import AdapterBatch
+    layer = Layer(adapters, rank, hidden, seed=hidden)
+    lengths, ids = [3, 20, 1, 9], [0, adapters - 1, -1, 0]
+    x, positions, rope = layer.inputs(33)
+    got = layer.prologue(x, positions, rope=rope, adapters=layer.adapters, batch=AdapterBatch(DEV, lengths, ids))
+    check(got, layer.expected(x, rope, lengths, ids))
+
+
+@pytest.mark.parametrize('tokens', [20, 400, 900])
+def test_a_broken_adapter_stays_with_its_request(tokens):
+    from qwen3_dspark_amd.adapters import AdapterBatch, QKVAdapters
+    layer = Layer(3, 8)
+    lengths = [tokens // 4] * 4
+    ids = [0, 1, -1, 2]
+    x, positions, rope = layer.inputs(tokens)
+    want = layer.prologue(x, positions, rope=rope, adapters=layer.adapters, batch=AdapterBatch(DEV, lengths, ids))
+    for p in 'qkv':
+        layer.a[p][1], layer.b[p][1] = float('nan'), float('inf')
+    broken = QKVAdapters(*(t for p in 'qkv' for t in (layer.a[p], layer.b[p])), scaling=layer.scaling)
+    got = layer.prologue(x, positions, rope=rope, adapters=broken, batch=AdapterBatch(DEV, lengths, ids))
+    mine = torch.arange(tokens, device=DEV) // (tokens // 4) == 1
+    for a, b in zip(got, want):
+        assert torch.equal(a[~mine], b[~mine]) and torch.isnan(a[mine]).all()
+    x[0] = float('inf')
+    got = layer.prologue(x, positions, rope=rope, adapters=layer.adapters, batch=AdapterBatch(DEV, lengths, ids))
+    for a, b in zip(got, want):
+        assert torch.equal(a[1:][~mine[1:]], b[1:][~mine[1:]]) and not torch.isfinite(a[0]).any()
+
+
+def test_no_adapter_in_the_batch():
+    from qwen3_dspark_amd.adapters import AdapterBatch
+    layer = Layer(2, 16)
+    x, positions, rope = layer.inputs(12)
+    got = layer.prologue(x, positions, rope=rope, adapters=layer.adapters, batch=AdapterBatch(DEV, [5, 7], [-1, -1]))
+    assert all(torch.equal(a, b) for a, b in zip(got, layer.prologue(x, positions, rope=rope)))
+
+
+def test_captured_and_replayed():
+    from qwen3_dspark_amd.adapters import AdapterBatch
+    layer = Layer(3, 16)
+    lengths, ids = [7] * 10, [i % 4 - 1 for i in range(10)]
+    batch = AdapterBatch(DEV, lengths, ids)
+    x, positions, rope = layer.inputs(70)
+    layer.prologue(x, positions, rope=rope, adapters=layer.adapters, batch=batch)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = layer.prologue(x, positions, rope=rope, adapters=layer.adapters, batch=batch)
+    for seed in range(3):
+        x.copy_(rnd(torch.Generator().manual_seed(seed), 70, H))
+        graph.replay()
+        eager = layer.prologue(x, positions, rope=rope, adapters=layer.adapters, batch=batch)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, eager))
+
+
+def test_two_streams():
+    from qwen3_dspark_amd.adapters import AdapterBatch
+    layer, other = Layer(3, 16), Layer(2, 64, seed=1)
+    lengths = [7] * 12
+    a = (layer, *layer.inputs(84), [i % 3 for i in range(12)])
+    b = (other, *other.inputs(84), [i % 2 for i in range(12)])
+    batches = [AdapterBatch(DEV, lengths, x[4]) for x in (a, b)]
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        got_a = [a[0].prologue(a[1], a[2], rope=a[3], adapters=a[0].adapters, batch=batches[0]) for _ in range(4)]
+    got_b = [b[0].prologue(b[1], b[2], rope=b[3], adapters=b[0].adapters, batch=batches[1]) for _ in range(4)]
+    torch.cuda.synchronize()
+    for got in got_a:
+        check(got, a[0].expected(a[1], a[3], lengths, a[4]))
+    for got in got_b:
+        check(got, b[0].expected(b[1], b[3], lengths, b[4]))
+
+
+def test_staged_in_a_transaction():
+    from qwen3_dspark_amd.adapters import AdapterBatch
+    from qwen3_dspark_amd.persistent_kv import Bucket, PersistentTargetKV
+    layer = Layer(2, 16)
+    store = PersistentTargetKV(layers=1, slots=3, context_capacity=64, max_query_tokens=24, heads=8, dim=128, device=DEV)
+    handles = [store.add_request(f'r{i}') for i in range(3)]
+    bucket = Bucket((8, 8, 8), (40, 40, 40), 'adapters')
+    store.register_bucket(bucket)
+    tx = store.begin(handles, bucket)
+    x, _, _ = layer.inputs(24)
+    batch = AdapterBatch(DEV, [8, 8, 8], [1, -1, 0])
+    q = store.stage_projected(tx, 0, x, layer.prologue, adapters=layer.adapters, batch=batch)
+    positions = store.workspace(bucket).positions
+    want = layer.prologue(x, positions, adapters=layer.adapters, batch=batch)
+    for got, w in zip((q, store.scratch_keys[0, :24], store.scratch_values[0, :24]), want):
+        assert torch.equal(got, w)
+
+
+def test_refusals():
+    from qwen3_dspark_amd.adapters import AdapterBatch, QKVAdapters
+    layer = Layer(2, 16)
+    x, positions, rope = layer.inputs(12)
+    batch = AdapterBatch(DEV, [5, 7], [0, 1])
+    with pytest.raises(ValueError, match='go together'):
+        layer.prologue(x, positions, adapters=layer.adapters)
+    with pytest.raises(ValueError, match='go together'):
+        layer.prologue(x, positions, batch=batch)
+    for other, match in ((AdapterBatch(DEV, [5, 6], [0, 1]), '12 tokens'), (AdapterBatch(DEV, [5, 7], [0, 2]), 'adapter 2 of 2')):
+        with pytest.raises(ValueError, match=match):
+            layer.prologue(x, positions, adapters=layer.adapters, batch=other)
+    with pytest.raises(ValueError, match='hidden size'):
+        layer.prologue(x, positions, adapters=Layer(2, 16, 256).adapters, batch=batch)
+    given = [t for p in 'qkv' for t in (layer.a[p], layer.b[p])]
+    for i, t, match in ((0, given[0].float(), 'bf16'), (1, given[1][:, :, :15], 'rank'), (2, given[2][:, :8], 'rank'),
+                        (3, given[3][:1], 'rank'), (5, given[1], 'rank')):
+        with pytest.raises(ValueError, match=match):
+            QKVAdapters(*given[:i], t, *given[i + 1:])
+    for scaling in (float('nan'), [1.0], [1.0, True]):
+        with pytest.raises(ValueError, match='scaling'):
+            QKVAdapters(*given, scaling=scaling)
