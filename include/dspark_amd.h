@@ -213,6 +213,29 @@ int dspark_mixed_attn_fwd(const void* q, const void* k, const void* v, const voi
                           int64_t workspace_bytes, void* stream);
 
 /*
+ * Attention of query tokens to a prefix that their requests share, for a call of
+ * dspark_mixed_attn_fwd behind it on the same stream: FP32 partials of the tokens over
+ * resident rows k0 .. k1 - 1 of one slot, all of them visible, left in the partial tiles
+ * that the mixed list reserves ahead of the requests' own segments (their records start at
+ * the prefix's end, and their request records count both).  No reference counterpart.
+ * k_res, v_res and strides as for dspark_verify_attn_fwd.  list (int32, device memory, 16-byte
+ * aligned, not validated beyond the bounds given here):
+ *   [0] the number of items, 7 ints unused
+ *   [max_items][8] items: slot, k0, k1 (k1 - k0 a multiple of 64), segment number, first token
+ *       record, token records (1 to 32), two unused
+ *   [max_tokens][4] tokens: query row, partial tile of segment 0, the token's place in it
+ *       (0 to 7), tiles from one segment to the next
+ * Members of the grid (a multiple of 8 workgroups, whose number modulo 8 is their KV head)
+ * walk the items; an empty list launches and leaves at once, so that a captured call
+ * serves lists to come.  workspace: dspark_attn_workspace_bytes(part_tiles, 0, 1, 32)
+ * bytes, the mixed call's.
+ */
+int dspark_prefix_attn_partials(const void* q, int64_t q_rows, const void* k_res, const void* v_res,
+                                int64_t slot_stride, int64_t tok_stride, int64_t head_stride, float scale,
+                                const int32_t* list, int max_items, int max_tokens, int workgroups, int part_tiles,
+                                void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
  * Multi-block DSpark draft attention.  Request r owns blocks
  * cu_blocks[r]..cu_blocks[r+1] (1..8 blocks), each 7 query rows; block b
  * sees context positions j < anchors[b] of its request plus its own 7 rows

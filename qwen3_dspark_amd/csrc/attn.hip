@@ -2083,6 +2083,197 @@ __global__ __launch_bounds__(PF_WAVES * WAVE, 2) void prefill_attn_kernel(Varlen
 }
 
 // ---------------------------------------------------------------------------
+// A prefix that many requests of a verification batch share (the same committed rows, of
+// which each keeps a copy): attended once for all of them
+// ---------------------------------------------------------------------------
+//   o = softmax([s_P, s_r]) [V_P; V_r], joined from the parts by (max, sum, O).
+//
+// The parts over a request's own keys are the runs and columns of a mixed list; here
+// the query tokens of a group of requests are attended to the group's prefix, split
+// along the keys, and leave FP32 partials in the requests' first partial slots, where
+// merge_kernel finds them.  Every query sees every key of the prefix, so there is no
+// mask, and cuts at multiples of 64 keys leave no partial stage.
+//
+// Work: a workgroup takes items (32 query tokens of a group, one key segment) of KV
+// head blockIdx.x % 8, which its XCD's L2 then holds for all of the group's token
+// tiles; the grid is fixed and the list says how many there are, so that a captured
+// launch serves every transaction.  Tiles and stages as in prefill_attn_kernel.
+struct PrefixArgs {
+  const bf16* q;           // [nq, 16, 128]
+  const bf16* k;           // resident layer
+  const bf16* v;
+  int64_t slot_stride, tok_stride, head_stride;
+  const int32_t* list;     // [8: item count], items [max_items][8], tokens [max_tokens][4]
+  float* part_o;
+  float* part_ml;
+  int max_items, max_tokens, part_tiles, q_rows;
+  float scale_log2;
+};
+
+__global__ __launch_bounds__(PF_WAVES * WAVE, 2) void prefix_attn_kernel(PrefixArgs a) {
+  __shared__ __attribute__((aligned(1024))) unsigned char smem[PF_SMEM];
+  const int g = blockIdx.x & 7;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int hh = lane >> 5;
+  const int n = lane & 31;
+  const int row0 = 16 * wave;
+  const uint32_t col[2] = {(uint32_t)(16 * ((lane & 15) ^ swz(row0 + (lane >> 4)))),
+                           (uint32_t)(16 * ((lane & 15) ^ swz(row0 + 8 + (lane >> 4))))};
+  const uint32_t off = (uint32_t)((lane >> 4) * a.tok_stride * 2);
+  const uint32_t smem_lds = lds_address(smem);
+  const TileOffsets co = ctx_tile_offsets<ROWB>(lane);
+  const int32_t* items = a.list + WORK_INTS;
+  const int32_t* tokens = items + WORK_INTS * a.max_items;
+  const int n_items = min(ld_const(a.list), a.max_items);
+  for (int it = blockIdx.x >> 3; it < n_items; it += gridDim.x >> 3) {
+    const int32_t* w = items + WORK_INTS * it;
+    const int slot = ld_const(w, 0), k0 = ld_const(w, 1), k1 = ld_const(w, 2), seg = ld_const(w, 3);
+    const int first = ld_const(w, 4), n_tok = min(ld_const(w, 5), min(PF_TOKENS, a.max_tokens - first));
+    if (n_tok < 1) continue;                                   // uniform
+    const int rg_log2 = n_tok <= PF_GROUP ? 0 : 1;
+    const int kg_count = PF_WAVES >> rg_log2;
+    const int rg = wave & ((1 << rg_log2) - 1);
+    const int kg = wave >> rg_log2;
+    const int tok = PF_GROUP * rg + (n >> 1);
+    const bool row_ok = tok < n_tok;
+    const int32_t* rec = tokens + 4 * (first + min(tok, n_tok - 1));
+    const int q_row = min(rec[0], a.q_rows - 1);
+    const int tile = rec[1] + seg * rec[3], sub = rec[2];
+
+    bf16x8 qf[8];
+    {
+      const bf16* qp = a.q + (size_t)q_row * Q_ROW + (size_t)(2 * g + (n & 1)) * HD + 8 * hh;
+      #pragma unroll
+      for (int ks = 0; ks < 8; ++ks) qf[ks] = ld8(qp + 16 * ks);
+    }
+    const size_t base = (size_t)slot * (size_t)a.slot_stride + (size_t)g * a.head_stride;
+    auto issue = [&](int step, bool is_v) {
+      const bf16* from = (is_v ? a.v : a.k) + base + (int64_t)(k0 + step * DSTEP + row0) * a.tok_stride;
+      const uint32_t to = smem_lds + (is_v ? PF_V : 0) + (uint32_t)((step & 1) * PF_HALF + wave * 4096);
+      #pragma unroll
+      for (int i = 0; i < 4; ++i)
+        lds_dma16_base(from + 4 * i * a.tok_stride, off + col[i >> 1], __builtin_amdgcn_readfirstlane(to + 1024u * i));
+    };
+    PairState st;
+    st.m = -INFINITY;
+    st.l = 0.f;
+    #pragma unroll
+    for (int D = 0; D < 4; ++D) st.o[D] = f32x16{};
+    const int n_steps = (k1 - k0) / DSTEP;
+    if (n_steps > 0) {
+      issue(0, false);
+      issue(0, true);
+      if (n_steps > 1) issue(1, false);
+    }
+    settle(qf[0], qf[1], qf[2], qf[3], qf[4], qf[5], qf[6], qf[7]);
+    const int h = kg & 1;
+    auto turn = [&](int s) { return ((2 * s) & (kg_count - 1)) == (kg & ~1); };
+    auto k_at = [&](int s) { return smem_lds + (uint32_t)((s & 1) * PF_HALF + 32 * h * ROWB) + co.k; };
+    auto v_at = [&](int s) { return smem_lds + (uint32_t)(PF_V + (s & 1) * PF_HALF + 32 * h * ROWB) + co.v; };
+    auto arrive = [&]() {
+      __builtin_amdgcn_sched_barrier(0);
+      load_wait<0>();
+      ring_barrier();
+    };
+    auto enter = [&](int s) {
+      arrive();
+      if (s + 1 < n_steps) issue(s + 1, true);
+      if (s + 2 < n_steps) issue(s + 2, false);
+    };
+    auto ahead = [&](int s) {
+      bf16x8 kf[8];
+      prefill_k(kf, k_at(s));
+      return prefill_scores(qf, kf);
+    };
+    f32x16 x = {};
+    int s = 0;
+    if (n_steps > 0) {
+      arrive();
+      if (turn(0)) x = ahead(0);
+    }
+    if (kg_count == 2) {
+      for (; s + 1 < n_steps; s += 2) {
+        enter(s);
+        const f32x16 y = prefill_full_tile(st, qf, x, k_at(s + 1), v_at(s), a.scale_log2);
+        enter(s + 1);
+        x = prefill_full_tile(st, qf, y, k_at(s + 2), v_at(s + 1), a.scale_log2);
+      }
+      if (s < n_steps) {
+        enter(s);
+        x = prefill_full_tile(st, qf, x, k_at(s + 1), v_at(s), a.scale_log2);
+        ++s;
+      }
+    }
+    for (; s < n_steps; ++s) {
+      enter(s);
+      if (turn(s)) {
+        const float m_use = prefill_max(st, x, a.scale_log2);
+        bf16x8 ph[2], pl[2];
+        prefill_probs(st, x, m_use, a.scale_log2, ph, pl);
+        #pragma unroll
+        for (int u = 0; u < 2; ++u)
+          #pragma unroll
+          for (int D = 0; D < 4; ++D) {
+            const bf16x8 vt = prefill_v(v_at(s), u, D);
+            st.o[D] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vt, ph[u], st.o[D], 0, 0, 0);
+            st.o[D] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vt, pl[u], st.o[D], 0, 0, 0);
+          }
+      }
+      if (turn(s + 1)) x = ahead(s + 1);
+    }
+    __syncthreads();   // every wave is done with the stages
+
+    // The key groups' states merge through LDS (as prefill_merge's) into the FP32 partial.
+    float* mb = reinterpret_cast<float*>(smem + wave * PF_STATE);
+    #pragma unroll
+    for (int D = 0; D < 4; ++D)
+      #pragma unroll
+      for (int q = 0; q < 4; ++q)
+        *reinterpret_cast<f32x4*>(mb + ((4 * D + q) * WAVE + lane) * 4) =
+            f32x4{st.o[D][4 * q], st.o[D][4 * q + 1], st.o[D][4 * q + 2], st.o[D][4 * q + 3]};
+    mb[64 * WAVE + lane] = st.m;
+    mb[65 * WAVE + lane] = st.l;
+    __syncthreads();
+    const float* group = reinterpret_cast<const float*>(smem + rg * PF_STATE);
+    const int next = (PF_STATE / 4) << rg_log2;
+    float m[4], M = -INFINITY, L = 0.f;
+    #pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      m[k] = k < kg_count ? group[k * next + 64 * WAVE + lane] : -INFINITY;
+      M = fmaxf(M, m[k]);
+    }
+    #pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      m[k] = m[k] == -INFINITY ? 0.f : fast_exp2(m[k] - M);
+      if (k < kg_count) L += m[k] * group[k * next + 65 * WAVE + lane];
+    }
+    L += __shfl_xor(L, 32);
+    if (row_ok && tile >= 0 && tile < a.part_tiles) {
+      const size_t row = ((size_t)tile * 8 + g) * 16 + 2 * (sub & 7) + (n & 1);
+      const int quads = 16 / kg_count;
+      for (int i = 0; i < quads; ++i) {
+        const int quad = kg * quads + i;
+        f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+        #pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          if (k >= kg_count) break;
+          const f32x4 y = *reinterpret_cast<const f32x4*>(group + k * next + (quad * WAVE + lane) * 4);
+          #pragma unroll
+          for (int e = 0; e < 4; ++e) acc[e] += y[e] * m[k];
+        }
+        *reinterpret_cast<f32x4*>(a.part_o + row * HD + 8 * quad + 4 * hh) = acc;
+      }
+      if (kg == 0 && hh == 0) {
+        a.part_ml[row * 2] = M;
+        a.part_ml[row * 2 + 1] = L;
+      }
+    }
+    __syncthreads();   // the next item's stages reuse the merge space
+  }
+}
+
+// ---------------------------------------------------------------------------
 // split-K merge: one workgroup per (request, KV head, tile) with >1 chunk
 // ---------------------------------------------------------------------------
 struct MergeArgs {
@@ -2432,6 +2623,34 @@ extern "C" int dspark_mixed_attn_fwd(const void* q, const void* k, const void* v
   if (rc != OK || part_tiles == 0) return rc;
   MergeArgs m{requests, nullptr, nullptr, nullptr, nullptr, a.part_o, a.part_ml, a.out, n_req, 0, 0, 0};
   return launch_merge(m, n_req, tiles, s);
+}
+
+extern "C" int dspark_prefix_attn_partials(const void* q, int64_t q_rows, const void* k_res, const void* v_res,
+                                           int64_t slot_stride, int64_t tok_stride, int64_t head_stride, float scale,
+                                           const int32_t* list, int max_items, int max_tokens, int workgroups,
+                                           int part_tiles, void* workspace, int64_t workspace_bytes_, void* stream) {
+  clear_error();
+  DSPARK_REQUIRE(q && k_res && v_res && list && workspace, "null pointer argument");
+  DSPARK_REQUIRE(aligned16(q) && aligned16(k_res) && aligned16(v_res) && aligned16(list) && aligned16(workspace),
+                 "Q/K/V, the list and the workspace must be 16-byte aligned");
+  DSPARK_REQUIRE(slot_stride >= 0 && tok_stride >= HD && tok_stride % 8 == 0 && head_stride >= HD && head_stride % 8 == 0,
+                 "resident strides must be multiples of 8 elements (token/head strides >= 128)");
+  DSPARK_REQUIRE(q_rows >= 1 && q_rows <= 0x7fffffffLL, "q_rows must be in [1, 2^31)");
+  DSPARK_REQUIRE(max_items >= 1 && max_tokens >= 1 && max_items <= (1 << 24) && max_tokens <= (1 << 26),
+                 "need max_items in [1, 2^24] and max_tokens in [1, 2^26]");
+  DSPARK_REQUIRE(workgroups >= 8 && workgroups % 8 == 0 && workgroups <= (1 << 20), "workgroups must be a multiple of 8 in [8, 2^20]");
+  DSPARK_REQUIRE(scale > 0.f && scale < 1e30f, "scale must be positive and finite");
+  DSPARK_REQUIRE(part_tiles >= 1, "part_tiles must be >= 1");
+  const int64_t need = dspark_attn_workspace_bytes(part_tiles, 0, 1, 32);
+  DSPARK_REQUIRE(workspace_bytes_ >= need, "workspace too small: %lld < %lld bytes", (long long)workspace_bytes_,
+                 (long long)need);
+  PrefixArgs a{static_cast<const bf16*>(q), static_cast<const bf16*>(k_res), static_cast<const bf16*>(v_res), slot_stride,
+               tok_stride, head_stride, list, static_cast<float*>(workspace), nullptr, max_items, max_tokens, part_tiles,
+               (int)q_rows, scale * LOG2E};
+  a.part_ml = a.part_o + (int64_t)part_tiles * HKV * 16 * HD;
+  hipLaunchKernelGGL(prefix_attn_kernel, dim3((unsigned)workgroups), dim3(PF_WAVES * WAVE), 0,
+                     static_cast<hipStream_t>(stream), a);
+  return launch_status("prefix_attn_kernel");
 }
 
 // ---------------------------------------------------------------------------

@@ -25,6 +25,7 @@ import torch
 from . import _native
 from ._device import KV_PAIR_SKEW, cu_count, kv_pair, require_gfx950, upload
 from .kernels import HEAD_DIM, KV_HEADS, SCALE
+from .shared_prefix import mixed_part_ints, shared_bytes, shared_capacity, shared_ints, shared_plan
 from .schedule import (DECODE_TOKENS, PART_TILE_BYTES, REQ_INTS, TILED_TOKENS, WORK_INTS, XCDS, check_chunk,
                        mixed_capacity, mixed_ints, mixed_plan, run_count, segment_plan, varlen_list_bound)
 
@@ -130,7 +131,7 @@ class HipKVDevice:
     """Resident and scratch KV in HBM plus the store's launches on gfx950."""
 
     def __init__(self, *, layers, slots, context_capacity, max_query_tokens, heads, dim, dtype, device, chunk,
-                 split, kv_skew=KV_PAIR_SKEW):
+                 split, kv_skew=KV_PAIR_SKEW, shared=False):
         # the copy kernels move 16-byte pieces of a head row
         if (dim * torch.empty((), dtype=dtype).element_size()) % 16:
             raise ValueError('A KV head row (dim * element size) must be a multiple of 16 bytes')
@@ -139,6 +140,7 @@ class HipKVDevice:
         self.layers, self.slots, self.capacity = layers, slots, context_capacity
         self.max_rows, self.heads, self.dim, self.dtype = max_query_tokens, heads, dim, dtype
         self.chunk, self.split = chunk, split
+        self.shared = shared           # plans attend rows that requests share once (shared_prefix)
         self.xcd_speed = None          # relative speed of each XCD for balanced plans (None: equal runs)
         self.slot_balance = True       # balanced plans give second-resident workgroups SECOND_SLOT_SHARE
         self.elem = torch.empty((), dtype=dtype).element_size()
@@ -176,6 +178,20 @@ class HipKVDevice:
                          if c is None else (c.run_records + c.prompt_records, c.runs, c.requests, c.columns, c.tiles))
         return ws.counts
 
+    def shared_counts(self, shape):
+        """SharedCapacity of a bucket's lists, where the store attends shared rows once."""
+        return shared_capacity(shape.request_count, shape.query_tokens, shape.maximum_query_length, cu_count(self.device))
+
+    def _list_ints(self, shape):
+        if self.shared:
+            return shared_ints(self.shared_counts(shape))
+        return _list_ints(shape, self.device, self.chunk, self.split)
+
+    def _partials_bytes(self, shape):
+        if self.shared:
+            return shared_bytes(self.shared_counts(shape))
+        return _partials_bytes(shape, self.device, self.chunk, self.split)
+
     # -- workspaces -----------------------------------------------------------
     def workspace(self, shape):
         """Allocate the buffers of a bucket, or of a family arena whose shape
@@ -191,17 +207,16 @@ class HipKVDevice:
             cu_key=torch.zeros(r + 1, dtype=torch.int32, device=d),
             positions=torch.zeros(q, dtype=torch.long, device=d),
             req=torch.zeros(3 * r, dtype=torch.int32, device=d),
-            work=torch.zeros(_list_ints(shape, d, self.chunk, self.split), dtype=torch.int32, device=d),
+            work=torch.zeros(self._list_ints(shape), dtype=torch.int32, device=d),
             keys=torch.empty((n, self.heads, self.dim), dtype=self.dtype, device=d),
             values=torch.empty((n, self.heads, self.dim), dtype=self.dtype, device=d),
-            attn=torch.zeros(_partials_bytes(shape, d, self.chunk, self.split), dtype=torch.uint8, device=d)))
+            attn=torch.zeros(self._partials_bytes(shape), dtype=torch.uint8, device=d)))
 
     def workspace_bytes(self, shape):
         """Exact allocation of workspace(shape), before allocating it."""
         n, r, q = shape.key_capacity, shape.request_count, shape.query_tokens
         kv = 2 * n * self.heads * self.dim * self.elem
-        return (kv + 18 * n + 8 * (r + 1) + 8 * q + 12 * r + 4 * _list_ints(shape, self.device, self.chunk, self.split)
-                + _partials_bytes(shape, self.device, self.chunk, self.split))
+        return (kv + 18 * n + 8 * (r + 1) + 8 * q + 12 * r + 4 * self._list_ints(shape) + self._partials_bytes(shape))
 
     # -- XCD calibration -------------------------------------------------------
     def measure_xcd_speed(self, workgroups=1024, passes=2):
@@ -222,14 +237,18 @@ class HipKVDevice:
                 self.values[:, slot, :n].detach().clone(memory_format=torch.contiguous_format))
 
     # -- one transaction --------------------------------------------------------
-    def build_metadata(self, ws, shape, slots, contexts, query_lengths):
+    def build_metadata(self, ws, shape, slots, contexts, query_lengths, groups=()):
         """Upload the request triples and the bucket's work list, then build
         the seven metadata arrays in one launch.  Raises before anything is
-        published if the list does not fit or a launch fails."""
+        published if the list does not fit or a launch fails.  groups: the prefixes that
+        requests of the batch share (a store that attends them once)."""
         key_lengths = [c + q for c, q in zip(contexts, query_lengths)]
         n_cu = cu_count(self.device)
-        capacity, counts = self.list_counts(ws, shape)
-        if capacity is not None:
+        capacity, counts = (None, None) if self.shared else self.list_counts(ws, shape)
+        if self.shared:
+            records = shared_plan(query_lengths, key_lengths, slots, groups, n_cu, self.shared_counts(shape),
+                                  xcd_speed=self.xcd_speed, slot_balance=self.slot_balance)
+        elif capacity is not None:
             records = mixed_plan(query_lengths, key_lengths, slots, n_cu, capacity=capacity, xcd_speed=self.xcd_speed,
                                  slot_balance=self.slot_balance).records
         else:
@@ -271,7 +290,15 @@ class HipKVDevice:
         time."""
         C = self.capacity
         k, v, sk, sv = self.layer_pointers[layer]
-        capacity, counts = self.list_counts(ws, shape)
+        if self.shared:
+            c = self.shared_counts(shape)
+            capacity, counts = c, (c.run_records + c.prompt_records, c.runs, c.requests, c.columns, c.tiles)
+            _native.call('dspark_prefix_attn_partials', query, shape.query_tokens, k, v, KV_HEADS * C * HEAD_DIM, HEAD_DIM,
+                         C * HEAD_DIM, SCALE, ws.work.data_ptr() + 4 * mixed_part_ints(c), c.items, c.tokens,
+                         8 * c.runs, c.tiles, ws.attn.data_ptr(), ws.attn.numel(),
+                         _native.stream_handle(self.device))
+        else:
+            capacity, counts = self.list_counts(ws, shape)
         if capacity is not None:
             check_chunk(self.chunk)
             n_work, runs, requests, columns, tiles = counts

@@ -33,6 +33,7 @@ import torch
 from .kernels import HEAD_DIM, KV_HEADS, Q_HEADS, SCALE, _check_scale
 from .kv_device import MAX_BUCKET_REQUESTS, HipKVDevice
 from .schedule import DEFAULT_CHUNK, SPLITS
+from .shared_prefix import inherited, shared_groups
 from .xcd import clipped, normalised
 
 
@@ -181,6 +182,7 @@ _POISONED = 'Store invalidated by copy failure; construct a new store'
 @dataclass
 class _Tenant:
     handle: Slot
+    lineage: tuple           # whose rows it holds (shared_prefix)
     length: int = 0
 
 
@@ -201,6 +203,7 @@ class _SlotLedger:
         self.vacant = list(range(slots))
         self.by_request = {}
         self.generation = 0
+        self.admitted = 0
 
     def admit(self, request):
         if not isinstance(request, str) or not request or request in self.by_request:
@@ -210,7 +213,8 @@ class _SlotLedger:
         i = heapq.heappop(self.vacant)
         self.incarnations[i] += 1
         handle = Slot(request, i, self.incarnations[i])
-        self.tenants[i] = _Tenant(handle)
+        self.admitted += 1
+        self.tenants[i] = _Tenant(handle, ((self.admitted, None),))
         self.by_request[request] = i
         self.generation += 1
         return handle
@@ -237,6 +241,14 @@ class _SlotLedger:
         for i, n in updates:
             self.tenants[i].length = n
         self.generation += 1
+
+    def lineage(self, i):
+        return self.tenants[i].lineage
+
+    def inherit(self, source, i, n):
+        """Tenant i's first n rows are now the source's."""
+        self.tenants[i].lineage = inherited(self.lineage(source), n, self.lineage(i)[-1][0])
+        self.set_lengths(((i, n),))
 
     def occupied(self):
         return len(self.by_request)
@@ -270,7 +282,7 @@ class PersistentTargetKV:
 
     def __init__(self, *, layers, slots, context_capacity, max_query_tokens,
                  heads, dim, dtype=torch.bfloat16, device='cuda', chunk=DEFAULT_CHUNK, split='balanced',
-                 kv_device=None):
+                 kv_device=None, shared_prefixes=False):
         dims = (layers, slots, context_capacity, max_query_tokens, heads, dim)
         if any(type(n) is not int or n < 1 for n in dims):
             raise ValueError('All capacities and dimensions must be positive integers')
@@ -278,15 +290,20 @@ class PersistentTargetKV:
             raise ValueError('Floating point KV dtype required')
         if split not in SPLITS:
             raise ValueError(f'split must be one of {SPLITS}')
+        if not isinstance(shared_prefixes, bool):
+            raise ValueError('shared_prefixes must be True or False')
+        if shared_prefixes and (split != 'balanced' or kv_device is not None):
+            raise ValueError('Shared prefixes need balanced plans on the store\'s own device half')
         if kv_device is None:
             kv_device = HipKVDevice(layers=layers, slots=slots, context_capacity=context_capacity,
                                     max_query_tokens=max_query_tokens, heads=heads, dim=dim, dtype=dtype,
-                                    device=device, chunk=int(chunk), split=split)
+                                    device=device, chunk=int(chunk), split=split,
+                                    shared=shared_prefixes)
         self.kv_device = kv_device
         self.device = kv_device.device
         self.layers, self.slot_capacity, self.context_capacity = layers, slots, context_capacity
         self.max_query_tokens, self.heads, self.dim, self.dtype = max_query_tokens, heads, dim, dtype
-        self.chunk, self.split = int(chunk), split
+        self.chunk, self.split, self.shared_prefixes = int(chunk), split, shared_prefixes
         self.keys, self.values = kv_device.keys, kv_device.values
         self.scratch_keys, self.scratch_values = kv_device.scratch_keys, kv_device.scratch_values
         self._phase = Phase.IDLE
@@ -406,6 +423,25 @@ class PersistentTargetKV:
             self._poison()
             raise
         self._ledger.set_lengths(((i, n),))
+
+    @torch.no_grad()
+    def share_prefix(self, source, handle, length):
+        """Give the empty slot of `handle` the first `length` committed rows of `source`, every
+        layer, without computing them again (no reference counterpart).  The slot keeps a
+        copy, so each request lives and ends on its own; a store built with
+        shared_prefixes=True remembers that the rows are the same, and a transaction's attention
+        reads them once for all of its requests that hold them.  Shared rows are those
+        that went from request to request by share_prefix, through any number of steps."""
+        self._permit('admin')
+        i, j = self._index(source), self._index(handle)
+        if type(length) is not int or not 0 <= length <= self._ledger.length(i) or i == j or self._ledger.length(j):
+            raise ValueError('Sharing requires an empty slot and committed rows of another request')
+        try:
+            self.kv_device.write_prefix(j, self.keys[:, i, :length], self.values[:, i, :length])
+        except Exception:
+            self._poison()
+            raise
+        self._ledger.inherit(i, j, length)
 
     def request_kv(self, handle):
         i = self._index(handle)
@@ -592,7 +628,9 @@ class PersistentTargetKV:
             raise ValueError('Actual context exceeds declared bucket applicability')
         if sum(contexts) + sum(query_lengths) >= 2 ** 31:
             raise ValueError('Varlen cumulative lengths exceed int32')
-        self.kv_device.build_metadata(self._workspaces[bucket], bucket, slots, contexts, query_lengths)
+        shared = ({'groups': shared_groups([self._ledger.lineage(i) for i in slots], contexts, slots)}
+                  if self.shared_prefixes else {})
+        self.kv_device.build_metadata(self._workspaces[bucket], bucket, slots, contexts, query_lengths, **shared)
         self._transactions += 1
         tx = Transaction(self._transactions, handles, contexts, bucket, query_lengths)
         self._phase, self._tx, self._tx_generation = nxt, tx, self._ledger.generation

@@ -1,0 +1,220 @@
+"""Which requests of a batch hold the same committed rows, and the plan that attends those
+rows once for all of them.
+
+Lineage.  The rows of a request are its own from some position on; the rows below were
+copied from another request (PersistentTargetKV.share_prefix).  A lineage lists, in order,
+(origin, end): rows up to `end` were written by `origin`, the last span (its own rows) having
+no end.  Committed rows never change, so two requests hold the same rows up to the
+position where their lineages part.
+
+Groups.  Requests with a common first origin are candidates for one group, which
+shares the rows that all of its members hold; members that would shorten it more than
+they gain stay out (shared_groups).
+
+Plan.  Runs and prompt columns over each request's own keys, as in a mixed plan
+(schedule.mixed_plan), whose records start at the prefix's end, with partial slots for the
+prefix's segments ahead of the request's own; and a list of prefix items
+(dspark_prefix_attn_partials in include/dspark_amd.h).  A request of a group always
+has partials, at least one of the prefix and one of its own keys.
+"""
+from collections import namedtuple
+
+import numpy as np
+
+from .schedule import (DECODE_TOKENS, PART_TILE_BYTES, PROMPT_TOKENS, REQ_INTS, RESIDENT_PER_CU, SEGMENT_COST, TILE, WORK_INTS,
+                       XCDS, _balanced_runs, _prompt_columns, prompt_segments, run_count, run_shares)
+
+PREFIX_TILE = 64              # prefixes end, and are cut, at multiples of this many keys (a ring stage)
+MIN_SHARED = 64               # fewest common rows that form a group
+MIN_PREFIX_SEGMENT = 256      # fewest keys of a prefix segment
+PREFIX_TILES = 1024           # partial tiles that prefix segments may take (more where one segment each needs it)
+TOKEN_INTS = 4
+
+SharedCapacity = namedtuple('SharedCapacity', 'run_records prompt_records runs requests columns tiles prefix_tiles items '
+                                              'tokens')
+Group = namedtuple('Group', 'members length slot')
+
+
+# -- lineages ---------------------------------------------------------------------
+def common_rows(a, b):
+    """Rows that two lineages have in common from the start (None: no end)."""
+    rows = 0
+    for (origin, end), (other, other_end) in zip(a, b):
+        if origin != other:
+            break
+        if end is None and other_end is None:
+            return None
+        rows = min(x for x in (end, other_end) if x is not None)
+        if end != other_end:
+            break
+    return rows
+
+
+def inherited(lineage, rows, origin):
+    """The lineage of `origin` with its first `rows` rows copied from `lineage`'s."""
+    spans = []
+    for at, end in lineage:
+        if rows <= (spans[-1][1] if spans else 0):
+            break
+        spans.append((at, rows if end is None else min(end, rows)))
+    return (*spans, (origin, None))
+
+
+def shared_groups(lineages, contexts, slots):
+    """[Group(members, rows, slot)] of a batch: the requests of each group hold
+    the same first `rows` rows, a multiple of PREFIX_TILE, which are read from `slot`."""
+    families = {}
+    for r, lineage in enumerate(lineages):
+        families.setdefault(lineage[0][0], []).append(r)
+    groups = []
+    for members in families.values():
+        # Everyone's lineage starts with the family's origin; rows in common with it all are
+        # the least of where the first spans end.
+        span = {r: min(contexts[r], contexts[r] if lineages[r][0][1] is None else lineages[r][0][1]) for r in members}
+        while len(members) > 1:
+            members.sort(key=lambda r: (-span[r], r))
+            best = max(range(2, len(members) + 1), key=lambda n: (n - 1) * (span[members[n - 1]] // PREFIX_TILE))
+            chosen = members[:best]
+            rows = span[chosen[-1]] // PREFIX_TILE * PREFIX_TILE
+            if rows < MIN_SHARED:
+                break
+            groups.append(Group(sorted(chosen), rows, slots[min(chosen)]))
+            members = members[best:]
+    return groups
+
+
+# -- plans ------------------------------------------------------------------------
+def _width(query_length):
+    """Partial tiles of a segment of a request."""
+    return -(-int(query_length) // DECODE_TOKENS)
+
+
+def shared_capacity(n_req, query_tokens, max_q, n_cu):
+    """The regions of a fixed-capacity shared list (SharedCapacity)."""
+    slots = max(XCDS, RESIDENT_PER_CU * n_cu // 8 // XCDS * XCDS)
+    prompts = max_q > DECODE_TOKENS
+    width = n_req + (query_tokens // DECODE_TOKENS if prompts else 0)
+    prefix = max(PREFIX_TILES, width)
+    own = width + n_req + slots + (PROMPT_TOKENS // DECODE_TOKENS * slots if prompts else 0)
+    tiles = query_tokens // PROMPT_TOKENS + n_req                      # 32-token tiles at most
+    return SharedCapacity(n_req + slots - 1, n_req + slots - 1 if prompts else 0, slots, n_req,
+                          max(slots, tiles) if prompts else 0, own + prefix, prefix, 2 * slots + tiles, query_tokens)
+
+
+def mixed_part_ints(c):
+    """int32 of the mixed list's part, whole 32-byte records."""
+    n = WORK_INTS * (c.run_records + c.prompt_records) + c.runs + 1 + REQ_INTS * c.requests + 2 * c.columns
+    return -(-n // WORK_INTS) * WORK_INTS
+
+
+def shared_ints(c):
+    """int32 length of a shared list: the mixed list, then the prefix items."""
+    return mixed_part_ints(c) + WORK_INTS * (1 + c.items) + TOKEN_INTS * c.tokens
+
+
+def shared_bytes(c):
+    return PART_TILE_BYTES * c.tiles
+
+
+def prefix_segments(tokens, rows, columns, room):
+    """Segments of a group's prefix: about `columns` (token tile, segment) items per KV
+    head, of at least MIN_PREFIX_SEGMENT keys, `room` at most."""
+    tiles = -(-tokens // PROMPT_TOKENS)
+    return max(1, min(columns // tiles, rows // MIN_PREFIX_SEGMENT, room))
+
+
+def shared_plan(query_lengths, key_lengths, starts, groups, n_cu, capacity, *, xcd_speed=None, slot_balance=True):
+    """The list of a batch whose `groups` share prefixes, laid out in the regions of
+    `capacity` (an int32 array)."""
+    c = capacity
+    n = len(query_lengths)
+    own_from = [0] * n
+    for group in groups:
+        for r in group.members:
+            own_from[r] = group.length
+    own = [k - f for k, f in zip(key_lengths, own_from)]
+    q0 = np.concatenate(([0], np.cumsum(query_lengths))).tolist()
+    width = [_width(q) for q in query_lengths]
+
+    # the prefixes' segments: the groups share the columns by their work, and the room for partials
+    per_head = max(XCDS, RESIDENT_PER_CU * n_cu // 8 // XCDS * XCDS)
+    work = [sum(query_lengths[r] for r in group.members) * group.length for group in groups]
+    least = sum(width[r] for group in groups for r in group.members)
+    parts, prefix_parts, items, tokens = [], [0] * n, [], []
+    for group, cost in zip(groups, work):
+        wide = sum(width[r] for r in group.members)
+        share = max(1, per_head * cost // sum(work))
+        room = max(1, c.prefix_tiles * wide // least // wide)
+        p = prefix_segments(sum(query_lengths[r] for r in group.members), group.length, share, room)
+        parts.append(p)
+        for r in group.members:
+            prefix_parts[r] = p
+
+    # the requests' own keys
+    decode = [r for r in range(n) if query_lengths[r] <= DECODE_TOKENS]
+    prompts = [r for r in range(n) if query_lengths[r] > DECODE_TOKENS]
+    groups_of_runs = min(run_count(sum(own[r] for r in decode) // (2 if prompts else 1), n_cu),
+                         max(XCDS, n_cu // 8 // XCDS * XCDS) if prompts else c.runs)
+    per_run = [[] for _ in range(XCDS)]
+    if decode:
+        per_run = [[(decode[r], a, b) for r, a, b in run]
+                   for run in _balanced_runs([own[r] for r in decode], groups_of_runs, TILE, SEGMENT_COST,
+                                             shares=run_shares(groups_of_runs, xcd_speed, n_cu if slot_balance else None))]
+    held = [0] * n
+    for run in per_run:
+        for r, _, _ in run:
+            held[r] += 1
+    taken = sum(p * width[r] for r, p in enumerate(prefix_parts)) + sum(held) + sum(width[r] for r in prompts)
+    loose = [(prompts[i], a, b) for i, a, b in
+             prompt_segments([query_lengths[r] for r in prompts], [own[r] for r in prompts],
+                             max(0, c.prompt_records - len(prompts)), n_cu, c.tiles - taken)]
+    segs = [x for run in per_run for x in run] + loose
+    for r, _, _ in loose:
+        held[r] += 1
+    slot, used = [-1] * n, 0
+    for r in range(n):
+        if prefix_parts[r] + held[r] > 1:
+            slot[r] = used
+            used += (prefix_parts[r] + held[r]) * width[r]
+    nxt = [s + p * w for s, p, w in zip(slot, prefix_parts, width)]
+    records = []
+    for r, a, b in segs:
+        at = -1
+        if slot[r] >= 0:
+            at, nxt[r] = nxt[r], nxt[r] + width[r]
+        records += (r, own_from[r] + a, own_from[r] + b, at, q0[r], query_lengths[r], key_lengths[r], starts[r])
+    requests = []
+    for r in range(n):
+        requests += (max(slot[r], 0), prefix_parts[r] + held[r], q0[r], query_lengths[r])
+    ranges = [0]
+    for run in per_run:
+        ranges.append(ranges[-1] + len(run))
+    first = ranges[-1]
+    rows = [(r, q0[r], query_lengths[r], key_lengths[r], starts[r]) for r in prompts]
+    place = {r: i for i, r in enumerate(prompts)}
+    columns = _prompt_columns(rows, [(place[r], own_from[r] + a, own_from[r] + b) for r, a, b in loose], c.run_records, True)
+
+    for group, p in zip(groups, parts):
+        start = len(tokens) // TOKEN_INTS
+        for r in group.members:
+            for t in range(query_lengths[r]):
+                tokens += (q0[r] + t, slot[r] + t // DECODE_TOKENS, t % DECODE_TOKENS, width[r])
+        count = len(tokens) // TOKEN_INTS - start
+        cuts = [i * (group.length // PREFIX_TILE) // p * PREFIX_TILE for i in range(p + 1)]
+        for i in range(p):
+            for t in range(0, count, PROMPT_TOKENS):
+                items += (group.slot, cuts[i], cuts[i + 1], i, start + t, min(PROMPT_TOKENS, count - t), 0, 0)
+
+    if (first > c.run_records or len(loose) > c.prompt_records or len(per_run) > c.runs or n > c.requests
+            or len(columns) > 2 * c.columns or used > c.tiles or len(items) > WORK_INTS * c.items
+            or len(tokens) > TOKEN_INTS * c.tokens):
+        raise ValueError('Segment plan exceeds its fixed capacity')
+    out = np.zeros(shared_ints(c), dtype=np.int32)
+    cut, n_work = WORK_INTS * first, c.run_records + c.prompt_records
+    after, base = WORK_INTS * n_work + c.runs + 1, mixed_part_ints(c)
+    for at, part in ((0, records[:cut]), (WORK_INTS * c.run_records, records[cut:]),
+                     (WORK_INTS * n_work, ranges + [first] * (c.runs - len(per_run))), (after, requests),
+                     (after + REQ_INTS * c.requests, columns), (base, [len(items) // WORK_INTS]), (base + WORK_INTS, items),
+                     (base + WORK_INTS * (1 + c.items), tokens)):
+        out[at:at + len(part)] = part
+    return out

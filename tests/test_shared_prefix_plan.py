@@ -1,0 +1,196 @@
+"""Lineages, groups and plans of requests that share committed rows (CPU): every plan
+covers each request's keys exactly once, its partial tiles are disjoint and within the
+capacity, and its regions hold what the kernels read."""
+import random
+
+import pytest
+import torch
+
+from kv_fake import store
+from qwen3_dspark_amd.schedule import REQ_INTS, WORK_INTS
+from qwen3_dspark_amd.shared_prefix import (PREFIX_TILE, common_rows, inherited, mixed_part_ints, shared_capacity,
+                                            shared_groups, shared_ints, shared_plan)
+
+
+def test_lineages():
+    a = ((1, None),)
+    b = inherited(a, 1000, 2)
+    d = inherited(b, 1500, 4)
+    assert b == ((1, 1000), (2, None)) and d == ((1, 1000), (2, 1500), (4, None))
+    assert inherited(b, 1000, 5) == ((1, 1000), (5, None)) and inherited(b, 700, 5) == ((1, 700), (5, None))
+    assert inherited(a, 0, 6) == ((6, None),)
+    assert [common_rows(*x) for x in ((a, b), (b, d), (a, d), (d, inherited(a, 300, 7)), (a, ((9, None),)))] == \
+        [1000, 1500, 1000, 300, 0]
+    assert common_rows(a, a) is None
+
+
+def rows_of(lineage, length):
+    """Who wrote each row."""
+    out = []
+    for origin, end in lineage:
+        out += [origin] * ((length if end is None else min(end, length)) - len(out))
+    return out
+
+
+def family(rng, n):
+    """Random requests: fresh ones, and ones that share rows of an earlier one."""
+    lineages, lengths = [], []
+    for r in range(n):
+        if lineages and rng.random() < 0.7:
+            s = rng.randrange(len(lineages))
+            rows = rng.randint(0, lengths[s])
+            lineages.append(inherited(lineages[s], rows, r))
+            lengths.append(rows + rng.choice((0, rng.randint(0, 900))))
+        else:
+            lineages.append(((r, None),))
+            lengths.append(rng.choice((0, rng.randint(0, 70), rng.randint(0, 5000))))
+    return lineages, lengths
+
+
+def check_plan(queries, keys, slots, groups, n_cu=256):
+    c = shared_capacity(len(queries), sum(queries), max(queries), n_cu)
+    out = shared_plan(queries, keys, slots, groups, n_cu, c).tolist()
+    assert len(out) == shared_ints(c) and mixed_part_ints(c) % 8 == 0
+    n_work = c.run_records + c.prompt_records
+    at = WORK_INTS * n_work
+    ranges = out[at:at + c.runs + 1]
+    requests = [out[at + c.runs + 1 + REQ_INTS * r:][:REQ_INTS] for r in range(c.requests)]
+    columns = out[at + c.runs + 1 + REQ_INTS * c.requests:][:2 * c.columns]
+    base = mixed_part_ints(c)
+    items = [out[base + 8 + 8 * i:][:8] for i in range(out[base])]
+    tokens = [out[base + 8 + 8 * c.items + 4 * i:][:4] for i in range(c.tokens)]
+    q0 = [sum(queries[:r]) for r in range(len(queries))]
+    width = [-(-q // 8) for q in queries]
+    covered = [[] for _ in queries]
+    tiles = [[] for _ in queries]
+
+    def own(rec, decode):
+        r, k0, k1, slot, row, q, k, start = rec
+        assert (row, q, k, start) == (q0[r], queries[r], keys[r], slots[r]) and (q <= 8) == decode
+        covered[r].append((k0, k1))
+        if slot >= 0:
+            tiles[r] += range(slot, slot + width[r])
+        else:
+            assert requests[r][1] == 1
+
+    assert ranges[0] == 0 and ranges == sorted(ranges) and ranges[-1] <= c.run_records
+    for i in range(ranges[-1]):
+        own(out[8 * i:8 * i + 8], True)
+    seen = set()
+    for i in range(0, len(columns), 2):
+        record, t = columns[i] - 1, columns[i + 1]
+        if record < 0:
+            continue
+        rec = out[8 * record:8 * record + 8]
+        assert 32 * t < rec[5] and (record, t) not in seen
+        seen.add((record, t))
+        if t == 0:
+            own(rec, False)
+    for record, _ in seen:
+        assert {t for x, t in seen if x == record} == set(range(-(-out[8 * record + 5] // 32)))
+    by_token = {}
+    for slot, k0, k1, seg, first, n, _, _ in items:
+        assert k0 % PREFIX_TILE == 0 and k1 % PREFIX_TILE == 0 and k0 < k1 and 1 <= n <= 32
+        for row, tile, sub, step in tokens[first:first + n]:
+            by_token.setdefault(row, []).append((k0, k1, tile + seg * step, sub, slot))
+    for r, q in enumerate(queries):
+        prefix = {tuple(sorted((k0, k1, slot) for k0, k1, _, _, slot in by_token.get(q0[r] + t, []))) for t in range(q)}
+        assert len(prefix) == 1
+        prefix = prefix.pop()
+        group = [g for g in groups if r in g.members]
+        if group:
+            assert prefix and {s for _, _, s in prefix} == {group[0].slot} and prefix[-1][1] == group[0].length
+        else:
+            assert not prefix
+        for t in range(q):
+            for _, _, tile, sub, _ in by_token.get(q0[r] + t, []):
+                assert sub == t % 8
+                if t % 8 == 0:
+                    tiles[r].append(tile)
+                else:
+                    assert tile in tiles[r]
+        spans = sorted([(a, b) for a, b, _ in prefix] + covered[r])
+        assert spans[0][0] == 0 and spans[-1][1] == keys[r] and all(x[1] == y[0] for x, y in zip(spans, spans[1:]))
+        first, count, row, rows = requests[r]
+        assert (row, rows) == (q0[r], q) and count == len(spans)
+        assert sorted(tiles[r]) == (list(range(first, first + count * width[r])) if count > 1 else [])
+    every = sorted(x for t in tiles for x in t)
+    assert len(set(every)) == len(every) and (not every or every[-1] < c.tiles)
+    return items
+
+
+@pytest.mark.parametrize('seed', range(40))
+def test_random_plans(seed):
+    rng = random.Random(seed)
+    n = rng.choice((1, 2, 3, 7, 20, 64))
+    lineages, contexts = family(rng, n)
+    longest = rng.choice((1, 8, 8, 40, 300))
+    queries = [rng.randint(1, longest) for _ in range(n)]
+    slots = rng.sample(range(100), n)
+    groups = shared_groups(lineages, contexts, slots)
+    members = [r for g in groups for r in g.members]
+    assert len(set(members)) == len(members)
+    for g in groups:
+        assert len(g.members) > 1 and g.length % PREFIX_TILE == 0 and 0 < g.length <= min(contexts[r] for r in g.members)
+        assert g.slot in [slots[r] for r in g.members]
+        assert len({tuple(rows_of(lineages[r], contexts[r])[:g.length]) for r in g.members}) == 1
+    check_plan(queries, [c + q for c, q in zip(contexts, queries)], slots, groups, rng.choice((256, 64, 304)))
+
+
+@pytest.mark.parametrize('n,q,rows,own', [(64, 1, 16384, 0), (64, 8, 100000, 5), (2, 1, 64, 0), (12, 400, 6000, 0),
+                                          (256, 7, 2048, 30), (2, 2000, 30000, 100), (1024, 2, 640, 1), (3, 9, 64, 0)])
+def test_large_and_small_plans(n, q, rows, own):
+    a = ((0, None),)
+    lineages = [inherited(a, rows, 1 + r) for r in range(n)]
+    groups = shared_groups(lineages, [rows + own] * n, list(range(n)))
+    assert [(len(g.members), g.length) for g in groups] == [(n, rows // 64 * 64)]
+    check_plan([q] * n, [rows + own + q] * n, list(range(n)), groups)
+
+
+def test_members_that_would_shorten_a_group_stay_out():
+    a = ((0, None),)
+    lineages = [a, inherited(a, 4000, 1), inherited(a, 4000, 2), inherited(a, 100, 3), inherited(a, 120, 4)]
+    groups = shared_groups(lineages, [5000, 4000, 4100, 100, 400], [4, 3, 2, 1, 0])
+    assert [(g.members, g.length, g.slot) for g in groups] == [([0, 1, 2], 3968, 4), ([3, 4], 64, 1)]
+    assert shared_groups(lineages[3:], [63, 400], [1, 0]) == []
+    assert shared_groups([a], [5000], [0]) == []
+
+
+def test_share_prefix_in_the_store():
+    pool = store(slots=4, context_capacity=24)
+    a, b, c, d = (pool.add_request(x) for x in 'abcd')
+    x = torch.randn(pool.layers, 9, pool.heads, pool.dim)
+    pool.load_prefix(a, x, x + 1)
+    pool.share_prefix(a, b, 7)
+    pool.share_prefix(b, c, 5)
+    assert [pool.length(h) for h in (a, b, c, d)] == [9, 7, 5, 0]
+    assert torch.equal(pool.request_kv(c)[0], x[:, :5]) and torch.equal(pool.request_kv(b)[1], x[:, :7] + 1)
+    assert common_rows(pool._ledger.lineage(a.index), pool._ledger.lineage(c.index)) == 5
+    for args in ((a, b, 3), (a, a, 0), (a, d, 10), (a, d, -1), (a, d, 2.0), (a, d, True), (d, d, 0)):
+        with pytest.raises(ValueError, match='empty slot'):
+            pool.share_prefix(*args)
+    pool.share_prefix(a, d, 0)
+    assert pool.length(d) == 0
+    pool.remove_request(a)
+    assert torch.equal(pool.request_kv(b)[0], x[:, :7])
+    with pytest.raises(ValueError, match='incarnation'):
+        pool.share_prefix(a, d, 1)
+    e = pool.add_request('e')
+    assert e.index == a.index and common_rows(pool._ledger.lineage(e.index), pool._ledger.lineage(b.index)) == 0
+    pool.kv_device.fail = 'write_prefix'
+    with pytest.raises(RuntimeError, match='injected'):
+        pool.share_prefix(b, d, 1)
+    assert pool.failed
+
+
+def test_constructor_refusals():
+    from kv_fake import CpuKVDevice
+    from qwen3_dspark_amd.persistent_kv import PersistentTargetKV
+    dims = dict(layers=1, slots=1, context_capacity=8, max_query_tokens=4, heads=8, dim=128)
+    for kw in (dict(split='request'), dict(kv_device=CpuKVDevice(**dims))):
+        with pytest.raises(ValueError, match='Shared prefixes need balanced'):
+            PersistentTargetKV(**dims, shared_prefixes=True, **kw)
+    with pytest.raises(ValueError, match='True or False'):
+        PersistentTargetKV(**dims, shared_prefixes=1)
+    with pytest.raises(RuntimeError, match='gfx950'):
+        PersistentTargetKV(**dims, shared_prefixes=True, device='cpu')
