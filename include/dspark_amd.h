@@ -458,26 +458,27 @@ int dspark_sample_rows(const double* probs, int rows, int vocab, const double* u
 /*
  * Sampling rules of the requests of a batch, applied to logits [rows, >= vocab]
  * (bf16 (dtype 0) or fp32 (1), row_stride elements apart) before a law is taken
- * from them; no reference counterpart.  Request r owns rows cu_rows[r] ..
- * cu_rows[r+1] (n_r + 1 rows, n_r <= 255 proposed tokens at tokens[cu_rows[r] -
+ * from them; no reference counterpart.  layout: int32 cu_rows [n_req + 1], then [3][n_req]:
+ * each request's row of history, the tokens it holds, how many of them are its prompt; in host
+ * memory with host_layout (at most 128 requests; read before the call returns),
+ * else in device memory.  Request r owns rows cu_rows[r] .. cu_rows[r+1] (n_r + 1 rows, n_r <= 255 proposed tokens at tokens[cu_rows[r] -
  * r ..], as dspark_spec_verify has them).  The text of its row j is its history and its
  * first j proposed tokens:
  *   y = x; if v occurs in the text, y = y > 0 ? y / rho : y * rho;
  *   y -= c alpha_f + [c > 0] alpha_p, c: occurrences behind the prompt;
  *   y += bias of v; and y = fill where the row's mask does not allow v.
- * text: int32 [3][n_req]: the request's row of history, the tokens it holds, how many
- * of them are its prompt.  history: int32 or int64 (history_bytes) rows, history_stride
+ * history: int32 or int64 (history_bytes) rows, history_stride
  * elements apart; tokens outside the vocabulary are passed over.  penalties:
  * double [3][n_req]: rho, alpha_p, alpha_f.  Biases of request r: entries bias_start[r] ..
- * bias_start[r+1] of bias_token / bias_value, no token twice.  allowed (optional):
+ * bias_start[r+1] of bias_token / bias_value, in ascending order of tokens, no token twice.  allowed (optional):
  * allowed_stride words a row, token v is bit v % 32 of word v / 32.  A row whose mask
  * allows no token is -infinity throughout.  A finite logit gives a finite value (clamped to
  * out's type) unless fill is not.  out: out_dtype dtype or 1; out may be logits itself
  * (same type and stride), and must not overlap it otherwise.  Arithmetic in 64 bits
  * on the values that change, rounded to out's type.
  */
-int dspark_logit_controls(const void* logits, int dtype, int64_t row_stride, int vocab, const int32_t* cu_rows,
-                          int n_req, const int32_t* text, const void* history, int history_bytes,
+int dspark_logit_controls(const void* logits, int dtype, int64_t row_stride, int vocab, const int32_t* layout,
+                          int host_layout, int n_req, const void* history, int history_bytes,
                           int64_t history_stride, const int64_t* tokens, const double* penalties,
                           const int32_t* bias_start, const int32_t* bias_token, const double* bias_value,
                           const int32_t* allowed, int64_t allowed_stride, float fill, void* out, int out_dtype,

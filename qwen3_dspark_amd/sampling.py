@@ -30,6 +30,7 @@ logits (and temperature overflow) and the uniforms are checked on the device
 and raise ValueError with the reference's messages after one device read.
 """
 import math
+from array import array
 from dataclasses import dataclass
 from numbers import Real
 
@@ -50,6 +51,7 @@ _ERRORS = {
     6: 'At most 255 proposed tokens per request',
 }
 MAX_PROPOSAL = 255
+_LAYOUT_ON_HOST = 128        # requests whose layout goes with the launch of the controls
 
 
 def validate_temperature(temperature):
@@ -216,10 +218,12 @@ class LogitControls:
         cu = [0]
         for x in counts:
             cu.append(cu[-1] + x + 1)
-        head = upload(self.device, cu + slots + lengths + prompts)
+        layout = array('i', cu + slots + lengths + prompts)
+        here = n <= _LAYOUT_ON_HOST
+        place = layout.buffer_info()[0] if here else (layout := upload(self.device, layout)).data_ptr()
         fill = torch.finfo(out.dtype).min if self.masked is None else self.masked
-        _native.call('dspark_logit_controls', logits.data_ptr(), dtype, logits.stride(0), self.vocab, head.data_ptr(), n,
-                     head[n + 1:].data_ptr(), history.data_ptr() or head.data_ptr(), history.element_size(),
+        _native.call('dspark_logit_controls', logits.data_ptr(), dtype, logits.stride(0), self.vocab, place, here, n,
+                     history.data_ptr() or logits.data_ptr(), history.element_size(),
                      history.stride(0), tokens.contiguous().data_ptr() if total else None, self._penalties.data_ptr(),
                      self._bias_start.data_ptr(), self._bias_token.data_ptr() or None, self._bias_value.data_ptr() or None,
                      None if allowed is None else allowed.data_ptr(), 0 if allowed is None else allowed.stride(0), fill,
