@@ -470,7 +470,7 @@ int dspark_sample_rows(const double* probs, int rows, int vocab, const double* u
  * history: int32 or int64 (history_bytes) rows, history_stride
  * elements apart; tokens outside the vocabulary are passed over.  penalties:
  * double [3][n_req]: rho, alpha_p, alpha_f.  Biases of request r: entries bias_start[r] ..
- * bias_start[r+1] of bias_token / bias_value, in ascending order of tokens, no token twice.  allowed (optional):
+ * bias_start[r+1] of bias_token / bias_value, at most 65,535, no token twice.  allowed (optional):
  * allowed_stride words a row, token v is bit v % 32 of word v / 32.  A row whose mask
  * allows no token is -infinity throughout.  A finite logit gives a finite value (clamped to
  * out's type) unless fill is not.  out: out_dtype dtype or 1; out may be logits itself

@@ -18,7 +18,6 @@
 
 namespace dspark {
 
-constexpr int LC_THREADS = 256;
 constexpr int LC_CHUNK = 4096;                   // tokens per workgroup
 constexpr int LC_PROPOSED = 255;                 // proposed tokens per request
 
@@ -46,7 +45,7 @@ struct ControlArgs {
   int32_t here[4 * LC_HERE + 1];
 };
 
-template <int T>
+template <int DT>
 struct LogitType;
 template <>
 struct LogitType<0> {
@@ -66,35 +65,50 @@ constexpr int LC_FLIGHT = 4;                     // 16-byte loads of a thread in
 template <int CH>
 struct ControlTables {
   uint32_t seen[CH];
-  uint16_t bias[CH];                             // 1 + the bias's entry behind the chunk's first, or 0
+  uint16_t bias[CH];                             // 1 + the request's entry, or 0
   uint32_t touched[CH / 32];                     // any of the above, or proposed
   uint32_t proposed[CH / 32];
   int32_t order[LC_PROPOSED + 1];                // the proposed tokens
   uint32_t allowed[LC_ROWS][CH / 32];            // of the rows at hand
   int32_t any[LC_ROWS];
-  int32_t first_bias;
 };
 
 template <int CH>
 __device__ __forceinline__ void mark(ControlTables<CH>& t, int at) { atomicOr(&t.touched[at >> 5], 1u << (at & 31)); }
 
-template <int CH, class Token>
+// Occurrences of the chunk's tokens in a text, 16 bytes of it per load where its rows allow it.
+template <int CH, int T, class Token>
 __device__ __forceinline__ void count_history(ControlTables<CH>& t, const Token* text, int held, int prompt, int v0, int n) {
   constexpr int BATCH = 8;
-  for (int i0 = threadIdx.x; i0 < held; i0 += LC_THREADS * BATCH) {
-    int64_t tok[BATCH];
+  constexpr int PER = 16 / (int)sizeof(Token);
+  typedef Token Pack __attribute__((ext_vector_type(PER)));
+  auto count = [&](Token token, int i) {
+    // other tokens, and numbers that are none, pass
+    const uint32_t at = (uint32_t)token - (uint32_t)v0;
+    if (at >= (uint32_t)n || (sizeof(Token) == 8 && (uint64_t)token >> 32)) return;
+    if (i < prompt) atomicOr(&t.seen[at], 0x80000000u);
+    else atomicAdd(&t.seen[at], 1u);
+    mark(t, (int)at);
+  };
+  const int packs = ((uintptr_t)text & 15) == 0 ? held / PER : 0;
+  for (int p0 = threadIdx.x; p0 < packs; p0 += T * BATCH) {
+    Pack pack[BATCH];
     #pragma unroll
-    for (int u = 0; u < BATCH; ++u) tok[u] = (int64_t)text[min(i0 + LC_THREADS * u, held - 1)];
+    for (int u = 0; u < BATCH; ++u) pack[u] = reinterpret_cast<const Pack*>(text)[min(p0 + T * u, packs - 1)];
     #pragma unroll
-    for (int u = 0; u < BATCH; ++u) {
-      const int i = i0 + LC_THREADS * u;
-      const int64_t at = tok[u] - v0;
-      if (i < held && at >= 0 && at < n) {       // other tokens, and numbers that are none, pass
-        if (i < prompt) atomicOr(&t.seen[at], 0x80000000u);
-        else atomicAdd(&t.seen[at], 1u);
-        mark(t, (int)at);
+    for (int u = 0; u < BATCH; ++u)
+      if (p0 + T * u < packs) {
+        #pragma unroll
+        for (int e = 0; e < PER; ++e) count(pack[u][e], PER * (p0 + T * u) + e);
       }
-    }
+  }
+  for (int i0 = PER * packs + threadIdx.x; i0 < held; i0 += T * BATCH) {
+    Token token[BATCH];
+    #pragma unroll
+    for (int u = 0; u < BATCH; ++u) token[u] = text[min(i0 + T * u, held - 1)];
+    #pragma unroll
+    for (int u = 0; u < BATCH; ++u)
+      if (i0 + T * u < held) count(token[u], i0 + T * u);
   }
 }
 
@@ -113,8 +127,8 @@ __device__ __forceinline__ uint32_t bits_from(const uint32_t* words, int at) {
 // the text, the logits.  The first logits are therefore loaded ahead of the text, the
 // rows' mask words are staged together, and a thread keeps LC_FLIGHT loads in flight,
 // over as many rows as it takes.
-template <int IN, int OUT, int CH, bool MASK>
-__global__ __launch_bounds__(LC_THREADS) void logit_controls_kernel(ControlArgs a) {
+template <int IN, int OUT, int CH, int T, bool MASK>
+__global__ __launch_bounds__(T) void logit_controls_kernel(ControlArgs a) {
   typedef typename LogitType<IN>::type In;
   typedef typename LogitType<OUT>::type Out;
   typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
@@ -148,7 +162,7 @@ __global__ __launch_bounds__(LC_THREADS) void logit_controls_kernel(ControlArgs 
     const int last = (n - 1) >> 5, bits = n - 32 * last;
     if (tid < LC_ROWS) t.any[tid] = 0;
     __syncthreads();
-    for (int i = tid; i < LC_ROWS * (CH / 32); i += LC_THREADS) {
+    for (int i = tid; i < LC_ROWS * (CH / 32); i += T) {
       const int j = i / (CH / 32), w = i % (CH / 32);
       if (j0 + j >= rows || w > last) continue;
       uint32_t x = a.allowed[(row0 + j0 + j) * a.allowed_stride + (v0 >> 5) + w];
@@ -176,25 +190,27 @@ __global__ __launch_bounds__(LC_THREADS) void logit_controls_kernel(ControlArgs 
   Group ready[LC_FLIGHT];
   auto fetch_all = [&](int j0, int count, int i) {
     #pragma unroll
-    for (int u = 0; u < LC_FLIGHT; ++u) fetch(j0, count, i + LC_THREADS * u, ready[u]);
+    for (int u = 0; u < LC_FLIGHT; ++u) fetch(j0, count, i + T * u, ready[u]);
   };
 
   if (MASK) stage_masks(0);
   {
-    if (tid == 0) t.first_bias = 0;
     u32x4* zero = reinterpret_cast<u32x4*>(&t);          // seen, bias, touched, proposed
-    for (int i = tid; i < (CH + CH / 2 + CH / 16) / 4; i += LC_THREADS) zero[i] = u32x4{0u, 0u, 0u, 0u};
+    for (int i = tid; i < (CH + CH / 2 + CH / 16) / 4; i += T) zero[i] = u32x4{0u, 0u, 0u, 0u};
   }
   __syncthreads();
   fetch_all(0, min(rows, LC_ROWS), tid);
   const int64_t first = (int64_t)text[r] * a.history_stride;
-  if (a.wide) count_history(t, static_cast<const int64_t*>(a.history) + first, held, prompt, v0, n);
-  else count_history(t, static_cast<const int32_t*>(a.history) + first, held, prompt, v0, n);
-  // The request's biases are sorted by token: those of the chunk follow one another.
+  if (a.wide) count_history<CH, T>(t, static_cast<const int64_t*>(a.history) + first, held, prompt, v0, n);
+  else count_history<CH, T>(t, static_cast<const int32_t*>(a.history) + first, held, prompt, v0, n);
   const int bias0 = a.bias_start[r], bias1 = a.bias_start[r + 1];
-  int below = 0;
-  for (int i = bias0 + tid; i < bias1; i += LC_THREADS) below += a.bias_token[i] < v0 ? 1 : 0;
-  if (below) atomicAdd(&t.first_bias, below);
+  for (int i = bias0 + tid; i < bias1; i += T) {
+    const int at = a.bias_token[i] - v0;
+    if (at >= 0 && at < n) {
+      t.bias[at] = (uint16_t)(1 + i - bias0);
+      mark(t, at);
+    }
+  }
   if (tid < n_prop) {
     const int64_t tok = a.tokens[row0 - r + tid];
     t.order[tid] = tok >= 0 && tok < a.vocab ? (int32_t)tok : -1;
@@ -205,15 +221,6 @@ __global__ __launch_bounds__(LC_THREADS) void logit_controls_kernel(ControlArgs 
     }
   }
   __syncthreads();
-  const int first_bias = bias0 + t.first_bias;
-  for (int i = first_bias + tid; i < min(bias1, first_bias + n); i += LC_THREADS) {
-    const int at = a.bias_token[i] - v0;
-    if (at >= 0 && at < n) {
-      t.bias[at] = (uint16_t)(1 + i - first_bias);
-      mark(t, at);
-    }
-  }
-  if (bias1 > bias0) __syncthreads();
   const double rho = a.penalties[r], inv_rho = 1.0 / rho, alpha_p = a.penalties[a.n_req + r], alpha_f = a.penalties[2 * a.n_req + r];
 
   auto control = [&](float x, int at, int j) {
@@ -224,7 +231,7 @@ __global__ __launch_bounds__(LC_THREADS) void logit_controls_kernel(ControlArgs 
     double y = (double)x;
     if (seen) y = y * (y > 0.0 ? inv_rho : rho);      // off by 2^-52 before the rounding to 24 bits
     if (c) y -= (double)c * alpha_f + alpha_p;
-    if (t.bias[at]) y += a.bias_value[first_bias + t.bias[at] - 1];
+    if (t.bias[at]) y += a.bias_value[bias0 + t.bias[at] - 1];
     // a finite logit stays finite
     if (fabsf(x) <= FLT_MAX) y = fmin(fmax(y, -(double)MOST), (double)MOST);
     return (float)y;
@@ -246,7 +253,7 @@ __global__ __launch_bounds__(LC_THREADS) void logit_controls_kernel(ControlArgs 
         const uint32_t* words = a.allowed + (row0 + j0 + j) * a.allowed_stride;
         const int last = (a.vocab - 1) >> 5, bits = a.vocab - 32 * last;
         uint32_t hit = 0;
-        for (int i = tid; i <= last; i += LC_THREADS) hit |= i == last && bits < 32 ? words[i] & ((1u << bits) - 1u) : words[i];
+        for (int i = tid; i <= last; i += T) hit |= i == last && bits < 32 ? words[i] & ((1u << bits) - 1u) : words[i];
         if (!__syncthreads_or(hit != 0u)) empty |= 1u << j;
       }
     }
@@ -279,14 +286,14 @@ __global__ __launch_bounds__(LC_THREADS) void logit_controls_kernel(ControlArgs 
         bf16x8 v;
         #pragma unroll
         for (int u = 0; u < 8; ++u) v[u] = (bf16)x[u % VEC];
-        *reinterpret_cast<bf16x8*>(to) = v;
+        __builtin_nontemporal_store(v, reinterpret_cast<bf16x8*>(to));
       } else {
         #pragma unroll
         for (int q = 0; q < VEC / 4; ++q)
-          *reinterpret_cast<f32x4*>(to + 4 * q) = f32x4{x[4 * q], x[4 * q + 1], x[4 * q + 2], x[4 * q + 3]};
+          __builtin_nontemporal_store(f32x4{x[4 * q], x[4 * q + 1], x[4 * q + 2], x[4 * q + 3]}, reinterpret_cast<f32x4*>(to + 4 * q));
       }
     };
-    for (int i = tid; i < count * GROUPS; i += LC_THREADS * LC_FLIGHT) {
+    for (int i = tid; i < count * GROUPS; i += T * LC_FLIGHT) {
       if (j0 || i != tid) fetch_all(j0, count, i);
       #pragma unroll
       for (int u = 0; u < LC_FLIGHT; ++u) finish(ready[u]);
@@ -297,7 +304,7 @@ __global__ __launch_bounds__(LC_THREADS) void logit_controls_kernel(ControlArgs 
       if (t.touched[at >> 5] >> (at & 31) & 1u) x = control(x, at, j0 + j);
       out_row(j0 + j)[at] = (Out)(keep ? x : empty >> j & 1u ? -INFINITY : a.fill);
     };
-    for (int i = tid; i < count * 2 * VEC; i += LC_THREADS) {       // at most VEC - 1 on either side
+    for (int i = tid; i < count * 2 * VEC; i += T) {       // at most VEC - 1 on either side
       const int j = i / (2 * VEC), e = i % (2 * VEC);
       const int lead = lead_of(j0 + j);
       if (e < VEC) {
@@ -309,7 +316,7 @@ __global__ __launch_bounds__(LC_THREADS) void logit_controls_kernel(ControlArgs 
     }
     for (int j = 0; j < count; ++j)
       if (lead_of(j0 + j) >= VEC)
-        for (int at = tid; at < n; at += LC_THREADS) single(j, at);
+        for (int at = tid; at < n; at += T) single(j, at);
   }
 }
 
@@ -319,12 +326,23 @@ using namespace dspark;
 
 namespace {
 
+// Up to so many workgroups (two per CU) take 512 threads, which shorten the chain of
+// each, and more of them 256, of which more fit a CU.  512 / 256 threads, us a launch: one row of
+// 151,936 4.7 / 5.3, 16 requests of up to 6 rows of 32,003 12.1 / 15.9; 64 requests of 8 rows of
+// 151,936 79.7 / 73.7, 32 FP32 rows over texts of up to 30,000 27.0 / 24.8.
+constexpr int LC_FEW = 512;
+
 template <int IN, int OUT>
 int launch_controls(const ControlArgs& a, hipStream_t s) {
   constexpr int CH = LC_CHUNK;
   const dim3 grid((unsigned)((a.vocab + CH - 1) / CH), (unsigned)a.n_req);
-  if (a.allowed) hipLaunchKernelGGL((logit_controls_kernel<IN, OUT, CH, true>), grid, dim3(LC_THREADS), 0, s, a);
-  else hipLaunchKernelGGL((logit_controls_kernel<IN, OUT, CH, false>), grid, dim3(LC_THREADS), 0, s, a);
+  if ((int64_t)grid.x * grid.y <= LC_FEW) {
+    if (a.allowed) hipLaunchKernelGGL((logit_controls_kernel<IN, OUT, CH, 512, true>), grid, dim3(512), 0, s, a);
+    else hipLaunchKernelGGL((logit_controls_kernel<IN, OUT, CH, 512, false>), grid, dim3(512), 0, s, a);
+  } else {
+    if (a.allowed) hipLaunchKernelGGL((logit_controls_kernel<IN, OUT, CH, 256, true>), grid, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((logit_controls_kernel<IN, OUT, CH, 256, false>), grid, dim3(256), 0, s, a);
+  }
   return launch_status("logit_controls_kernel");
 }
 

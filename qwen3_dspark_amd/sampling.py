@@ -32,7 +32,9 @@ and raise ValueError with the reference's messages after one device read.
 import math
 from array import array
 from dataclasses import dataclass
+from itertools import accumulate, repeat
 from numbers import Real
+from operator import add, gt
 
 import torch
 
@@ -51,6 +53,7 @@ _ERRORS = {
     6: 'At most 255 proposed tokens per request',
 }
 MAX_PROPOSAL = 255
+_LOWEST = {t: torch.finfo(t).min for t in (torch.bfloat16, torch.float32)}
 _LAYOUT_ON_HOST = 128        # requests whose layout goes with the launch of the controls
 
 
@@ -136,6 +139,8 @@ class LogitControls:
             rules += [float(p) for p in x]
         start, tokens, values = [0], [], []
         for d in [None] * n if bias is None else bias:
+            if len(d or {}) > 65535:
+                raise ValueError('At most 65,535 biases per request')
             for token, value in sorted((d or {}).items()):
                 if type(token) is not int or not 0 <= token < vocab:
                     raise ValueError('Biased tokens must be integers in the vocabulary')
@@ -153,11 +158,11 @@ class LogitControls:
         self._bias_start = upload(self.device, start)
         self._bias_token = upload(self.device, tokens)
         self._bias_value = upload(self.device, values, torch.float64)
-        self._stream = torch.cuda.current_stream(self.device)
+        self._stream = _native.stream_handle(self.device)
         self._uploaded = torch.cuda.Event()
-        self._uploaded.record(self._stream)
+        self._uploaded.record(torch.cuda.current_stream(self.device))
+        self._none, self._each = array('i', [0] * n), array('i', range(n))
 
-    @torch.no_grad()
     def __call__(self, logits, history, *, lengths, prompt_lengths=None, counts=None, tokens=None, slots=None,
                  allowed=None, out=None):
         """logits [rows, vocab] bf16 or fp32, request-major; history: int32 or int64
@@ -173,33 +178,34 @@ class LogitControls:
             raise ValueError(f'Logits must be [rows, {self.vocab}] on the controls\' device')
         if torch.cuda.is_current_stream_capturing():
             raise ValueError('The lengths are uploaded with each call, which a captured graph cannot repeat')
-        lengths = [int(x) for x in lengths]
-        n = len(lengths)
-        prompts = [0] * n if prompt_lengths is None else [int(x) for x in prompt_lengths]
-        counts = [0] * n if counts is None else [int(x) for x in counts]
-        slots = list(range(n)) if slots is None else [int(x) for x in slots]
-        if n != self.requests:
-            raise ValueError(f'These controls rule {self.requests} requests')
+        n = self.requests
+        lengths = array('i', lengths)
+        prompts = self._none if prompt_lengths is None else array('i', prompt_lengths)
+        counts = self._none if counts is None else array('i', counts)
+        slots = self._each if slots is None else array('i', slots)
+        if len(lengths) != n:
+            raise ValueError(f'These controls rule {n} requests')
         if not len(prompts) == len(counts) == len(slots) == n:
             raise ValueError('One length, prompt length, proposal length and text per request required')
-        if any(x < 0 for x in counts) or len(logits) != sum(counts) + n:
+        rows, total = len(logits), sum(counts)
+        if min(counts) < 0 or rows != total + n:
             raise ValueError('Each request has a row for each of its proposed tokens and one more')
         if max(counts) > MAX_PROPOSAL:
             raise ValueError(_ERRORS[6])
         if (not isinstance(history, torch.Tensor) or history.ndim != 2 or history.device != self.device
                 or history.dtype not in (torch.int32, torch.int64) or history.stride(1) != 1 and history.shape[1] > 1):
             raise ValueError('history must be int32 or int64 [texts, capacity] with contiguous rows')
-        if any(not 0 <= s < len(history) for s in slots) \
-                or any(not 0 <= p <= x <= history.shape[1] for p, x in zip(prompts, lengths)):
+        texts, capacity = history.shape
+        if (min(slots) < 0 or max(slots) >= texts or min(prompts) < 0 or max(lengths) > capacity
+                or any(map(gt, prompts, lengths))):
             raise ValueError('Texts must lie within history, prompts within their texts')
-        total = sum(counts)
         if total and (not isinstance(tokens, torch.Tensor) or tokens.dtype != torch.long or tokens.shape != (total,)
                       or tokens.device != self.device):
             raise ValueError('tokens must be the proposed tokens, int64, on the controls\' device')
         words = (self.vocab + 31) // 32
         if allowed is not None and (
                 not isinstance(allowed, torch.Tensor) or allowed.dtype != torch.int32 or allowed.device != self.device
-                or allowed.ndim != 2 or allowed.shape[0] != len(logits) or allowed.shape[1] < words
+                or allowed.ndim != 2 or allowed.shape[0] != rows or allowed.shape[1] < words
                 or allowed.stride(1) != 1 or allowed.stride(0) < words):
             raise ValueError('allowed must be int32 [rows, ceil(vocab / 32)] with contiguous rows')
         if out is None:
@@ -212,22 +218,19 @@ class LogitControls:
             raise ValueError('out must be the logits or not overlap them')
         if logits.stride(0) < self.vocab:
             raise ValueError('Logit rows must not overlap')
-        stream = torch.cuda.current_stream(self.device)
+        stream = _native.stream_handle(self.device)
         if stream != self._stream:
-            stream.wait_event(self._uploaded)
-        cu = [0]
-        for x in counts:
-            cu.append(cu[-1] + x + 1)
-        layout = array('i', cu + slots + lengths + prompts)
+            torch.cuda.current_stream(self.device).wait_event(self._uploaded)
+        layout = array('i', accumulate(map(add, counts, repeat(1)), initial=0)) + slots + lengths + prompts
         here = n <= _LAYOUT_ON_HOST
         place = layout.buffer_info()[0] if here else (layout := upload(self.device, layout)).data_ptr()
-        fill = torch.finfo(out.dtype).min if self.masked is None else self.masked
+        fill = _LOWEST[out.dtype] if self.masked is None else self.masked
         _native.call('dspark_logit_controls', logits.data_ptr(), dtype, logits.stride(0), self.vocab, place, here, n,
                      history.data_ptr() or logits.data_ptr(), history.element_size(),
                      history.stride(0), tokens.contiguous().data_ptr() if total else None, self._penalties.data_ptr(),
                      self._bias_start.data_ptr(), self._bias_token.data_ptr() or None, self._bias_value.data_ptr() or None,
                      None if allowed is None else allowed.data_ptr(), 0 if allowed is None else allowed.stride(0), fill,
-                     out.data_ptr(), 0 if out.dtype == torch.bfloat16 else 1, out.stride(0), stream.cuda_stream)
+                     out.data_ptr(), 0 if out.dtype == torch.bfloat16 else 1, out.stride(0), stream)
         return out
 
 
