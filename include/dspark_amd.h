@@ -461,7 +461,8 @@ int dspark_sample_rows(const double* probs, int rows, int vocab, const double* u
  * from them; no reference counterpart.  layout: int32 cu_rows [n_req + 1], then [3][n_req]:
  * each request's row of history, the tokens it holds, how many of them are its prompt; in host
  * memory with host_layout (at most 128 requests; read before the call returns),
- * else in device memory.  Request r owns rows cu_rows[r] .. cu_rows[r+1] (n_r + 1 rows, n_r <= 255 proposed tokens at tokens[cu_rows[r] -
+ * else in device memory.  rows and text_tokens: of all
+ * requests, by which the work is cut.  Request r owns rows cu_rows[r] .. cu_rows[r+1] (n_r + 1 rows, n_r <= 255 proposed tokens at tokens[cu_rows[r] -
  * r ..], as dspark_spec_verify has them).  The text of its row j is its history and its
  * first j proposed tokens:
  *   y = x; if v occurs in the text, y = y > 0 ? y / rho : y * rho;
@@ -478,7 +479,7 @@ int dspark_sample_rows(const double* probs, int rows, int vocab, const double* u
  * on the values that change, rounded to out's type.
  */
 int dspark_logit_controls(const void* logits, int dtype, int64_t row_stride, int vocab, const int32_t* layout,
-                          int host_layout, int n_req, const void* history, int history_bytes,
+                          int host_layout, int n_req, int64_t rows, int64_t text_tokens, const void* history, int history_bytes,
                           int64_t history_stride, const int64_t* tokens, const double* penalties,
                           const int32_t* bias_start, const int32_t* bias_token, const double* bias_value,
                           const int32_t* allowed, int64_t allowed_stride, float fill, void* out, int out_dtype,

@@ -67,7 +67,7 @@ SIGNATURES = {
     'dspark_spec_verify': (_I, [_P, _I, _L, _I, _D, _P, _P, _P, _I, _P, _P, _P, _P, _P, _I, _P, _P, _P, _L, _P]),
     'dspark_logits_to_probs': (_I, [_P, _I, _I, _I, _L, _D, _P, _P, _P]),
     'dspark_sample_rows': (_I, [_P, _I, _I, _P, _P, _P, _L, _P]),
-    'dspark_logit_controls': (_I, [_P, _I, _L, _I, _P, _I, _I, _P, _I, _L, _P, _P, _P, _P, _P, _P, _L, _F, _P, _I, _L,
+    'dspark_logit_controls': (_I, [_P, _I, _L, _I, _P, _I, _I, _L, _L, _P, _I, _L, _P, _P, _P, _P, _P, _P, _L, _F, _P, _I, _L,
                                    _P]),
     'dspark_crop_plan_workspace_bytes': (_L, [_L]),
     'dspark_crop_plan': (_I, [_P, _P, _L, _L, _L, _P, _P, _P, _P, _L, _P]),

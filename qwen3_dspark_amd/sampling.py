@@ -225,7 +225,7 @@ class LogitControls:
         here = n <= _LAYOUT_ON_HOST
         place = layout.buffer_info()[0] if here else (layout := upload(self.device, layout)).data_ptr()
         fill = _LOWEST[out.dtype] if self.masked is None else self.masked
-        _native.call('dspark_logit_controls', logits.data_ptr(), dtype, logits.stride(0), self.vocab, place, here, n,
+        _native.call('dspark_logit_controls', logits.data_ptr(), dtype, logits.stride(0), self.vocab, place, here, n, rows, sum(lengths),
                      history.data_ptr() or logits.data_ptr(), history.element_size(),
                      history.stride(0), tokens.contiguous().data_ptr() if total else None, self._penalties.data_ptr(),
                      self._bias_start.data_ptr(), self._bias_token.data_ptr() or None, self._bias_value.data_ptr() or None,

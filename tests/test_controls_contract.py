@@ -33,14 +33,14 @@ def test_entry_point_checks():
     fake = ctypes.c_void_p(1 << 20)                # never dereferenced
 
     def call(**kw):
-        args = dict(logits=fake, dtype=0, row_stride=100, vocab=100, layout=fake, host_layout=0, n_req=1, history=fake,
+        args = dict(logits=fake, dtype=0, row_stride=100, vocab=100, layout=fake, host_layout=0, n_req=1, rows=1, text_tokens=0, history=fake,
                     history_bytes=8, history_stride=4, tokens=fake, penalties=fake, bias_start=fake, bias_token=fake,
                     bias_value=fake, allowed=fake, allowed_stride=4, fill=0.0, out=ctypes.c_void_p(1 << 21), out_dtype=0,
                     out_stride=100, stream=None)
         args.update(kw)
         return lib.dspark_logit_controls(*args.values()), lib.dspark_last_error().decode()
     for kw, match in ((dict(logits=None), 'null'), (dict(history=None), 'null'), (dict(n_req=0), 'n_req'),
-                      (dict(n_req=65536), 'n_req'), (dict(layout=None), 'null'),
+                      (dict(n_req=65536), 'n_req'), (dict(layout=None), 'null'), (dict(rows=0), 'rows'), (dict(text_tokens=-1), 'rows'),
                       (dict(host_layout=1, n_req=129), 'host memory'), (dict(vocab=0), 'vocab'), (dict(row_stride=99), 'vocab'),
                       (dict(out_stride=99), 'vocab'), (dict(dtype=2), 'dtype'), (dict(dtype=1), 'out_dtype'),
                       (dict(history_bytes=2), 'history'), (dict(history_stride=-1), 'mask row'),
