@@ -17,7 +17,6 @@ from numbers import Real
 
 import torch
 
-from . import _native
 from ._device import require_gfx950, upload
 from .kernels import HEAD_DIM, KV_HEADS, Q_HEADS
 
@@ -77,7 +76,7 @@ class QKVAdapters:
             raise ValueError('scaling must be a finite number, or one per adapter')
         self.device = require_gfx950(a_q.device)
         self.count, self.rank, self.hidden = n, rank, hidden
-        self.padded_rank = -(-rank // 16) * 16
+        self.padded_rank = 16 if rank <= 16 else 32 if rank <= 32 else -(-rank // 64) * 64      # what the kernels take
         self.a = torch.zeros((n, 3, self.padded_rank, hidden), dtype=torch.bfloat16, device=self.device)
         self.b = torch.zeros((n, q + 2 * kv, self.padded_rank), dtype=torch.bfloat16, device=self.device)
         for i, t in enumerate((a_q, a_k, a_v)):
@@ -85,6 +84,7 @@ class QKVAdapters:
         for at, t in ((0, b_q), (q, b_k), (q + kv, b_v)):
             self.b[:, at:at + t.shape[1], :rank] = t.detach()
         self.scaling = upload(self.device, [float(x) for x in scaling], torch.float32)
+        self.pointers = (self.a.data_ptr(), self.b.data_ptr(), self.scaling.data_ptr(), n, self.padded_rank, rank)
 
     def check(self, batch, tokens, hidden, device):
         """Refuse a batch or prologue that these adapters do not fit."""
@@ -95,10 +95,6 @@ class QKVAdapters:
         if batch.largest >= self.count:
             raise ValueError(f'The batch names adapter {batch.largest} of {self.count}')
 
-    def shrink(self, hidden, batch):
-        """scaling A x of every token that has an adapter, as the adapted prologue takes it."""
-        u = torch.empty((3, batch.tokens, 2, self.padded_rank), dtype=torch.bfloat16, device=self.device)
-        _native.call('dspark_adapter_shrink', hidden.data_ptr(), batch.tokens, self.hidden, self.a.data_ptr(),
-                     self.scaling.data_ptr(), self.count, self.padded_rank, self.rank, batch.tiles.data_ptr(),
-                     batch.n_tiles, u.data_ptr(), _native.stream_handle(self.device))
-        return u
+    def scratch(self, tokens):
+        """Elements of the scaled A x of a batch, two bf16 numbers each."""
+        return 3 * tokens * 2 * self.padded_rank

@@ -45,26 +45,29 @@ struct PrologueArgs {
 };
 
 // grid: 32 heads (0-15 q, 16-23 k, 24-31 v) x ceil(T / (32 TG)) token tiles, one
-// dimension (see the XCD mapping below); 4 TG waves.  ADAPT: with low-rank adapters.
-template <int TG, bool ADAPT = false>
+// dimension (see the XCD mapping below); 4 TG waves.  RK: with low-rank adapters, in tiles
+// of ad.tile_tokens (adapters.h).
+template <int TG, int RK = 0>
 __global__ __launch_bounds__(4 * TG * WAVE) void qkv_prologue_kernel(PrologueArgs a, AdapterArgs ad) {
   __shared__ __attribute__((aligned(16))) unsigned char smem[HeadRing<TG>::SMEM];
   // XCD-aware placement: workgroups are dealt round-robin over the 8 XCDs
   // (each with its own L2), so the token tiles of one head are given ids
   // that share id % 8 - the head's weight slice is then fetched from HBM by
   // one L2 and served to all of its tiles from there.
-  const int tiles = (a.tokens + 32 * TG - 1) / (32 * TG);
+  const int per_tile = RK ? ad.tile_tokens : 32 * TG;
+  const int tiles = (a.tokens + per_tile - 1) / per_tile;
   const int xcd = blockIdx.x & 7;
   const int slot = blockIdx.x >> 3;
   const int head = xcd + 8 * (slot / tiles);
-  const int t0 = (slot % tiles) * (32 * TG);
+  const int t0 = (slot % tiles) * per_tile;
+  const int end = min(t0 + per_tile, a.tokens);
   const int kind = head < HQ ? 0 : (head < HQ + HKV ? 1 : 2);       // workgroup-uniform
   const int hh = kind == 0 ? head : (kind == 1 ? head - HQ : head - HQ - HKV);
   const bf16* w = (kind == 0 ? a.wq : (kind == 1 ? a.wk : a.wv)) + (size_t)hh * HD * a.hidden;
 
   const HeadLaneOf<TG> L;
   const int row = t0 + L.token();
-  const int tok = min(row, a.tokens - 1);
+  const int tok = min(row, end - 1);
   HeadNormWOf<TG> nw;
   HeadRopeOf<TG> rope;
   float pos = 0.f;
@@ -78,12 +81,12 @@ __global__ __launch_bounds__(4 * TG * WAVE) void qkv_prologue_kernel(PrologueArg
       else pos = (float)a.positions[tok];
     }
   };
-  if constexpr (ADAPT) {
-    head_tile_gemm<false, TG>(w, a.x, a.tokens, a.hidden, t0, smem, v, ss, fetch, [&](f32x16 (&acc)[2]) {
-      const int id[1] = {ad.token[tok]};
-      const bf16* const u[1] = {ad.u + ((size_t)kind * a.tokens + tok) * 2 * ad.rank};
-      adapter_expand<1>([&](int i, int) -> f32x16& { return acc[i]; }, ad, head, id, u,
-                        [&](int i) { return 32 * (L.dh + 2 * i) + L.n; }, L.kq, 2);
+  if constexpr (RK != 0) {
+    const int id[1] = {ad.token[tok]};
+    const bf16* const u[1] = {ad.u + ((size_t)kind * a.tokens + tok) * 2 * ad.rank};
+    head_tile_gemm<false, TG>(w, a.x, end, a.hidden, t0, smem, v, ss, fetch, [&](f32x16 (&acc)[2]) {
+      adapter_expand<1, RK, 2>([&](int i, int) -> f32x16& { return acc[i]; }, ad, head, id, u,
+                               [&](int i) { return 32 * (L.dh + 2 * i) + L.n; }, L.kq);
     });
   } else {
     head_tile_gemm<false, TG>(w, a.x, a.tokens, a.hidden, t0, smem, v, ss, fetch);
@@ -94,11 +97,11 @@ __global__ __launch_bounds__(4 * TG * WAVE) void qkv_prologue_kernel(PrologueArg
     head_rope(v, rope);
   }
   bf16* out = kind == 0 ? a.q_out + (size_t)tok * Q_ROW : (kind == 1 ? a.k_out : a.v_out) + (size_t)tok * a.kv_row_stride;
-  head_store<TG>(v, out + (size_t)hh * HD, row < a.tokens);
+  head_store<TG>(v, out + (size_t)hh * HD, row < end);
 }
 
 // The same for many tokens: 128-token tiles (wide_gemm.h), two workgroups per CU.
-template <bool TABLE, bool ADAPT = false>
+template <bool TABLE, int RK = 0>
 __global__ __launch_bounds__(WG_WAVES * WAVE, 2) void qkv_prologue_wide_kernel(PrologueArgs a, AdapterArgs ad) {
   __shared__ __attribute__((aligned(16))) unsigned char smem[WG_SMEM];
   const int tiles = (a.tokens + WG_TOKENS - 1) / WG_TOKENS;
@@ -112,7 +115,7 @@ __global__ __launch_bounds__(WG_WAVES * WAVE, 2) void qkv_prologue_wide_kernel(P
   f32x16 v[2][2];
   wide_tile_gemm(w, a.x, a.tokens, a.hidden, t0, smem, v);
   const WideLane L;
-  if constexpr (ADAPT) {
+  if constexpr (RK != 0) {
     int id[2];
     const bf16* u[2];
     #pragma unroll
@@ -122,8 +125,8 @@ __global__ __launch_bounds__(WG_WAVES * WAVE, 2) void qkv_prologue_wide_kernel(P
       u[tt] = ad.u + ((size_t)kind * a.tokens + tok) * 2 * ad.rank;
     }
     const bf16* const uc[2] = {u[0], u[1]};
-    adapter_expand<2>([&](int i, int tt) -> f32x16& { return v[i][tt]; }, ad, head, id, uc,
-                      [&](int i) { return 32 * (L.dh + 2 * i) + L.n; }, 0, 1);
+    adapter_expand<2, RK, 1>([&](int i, int tt) -> f32x16& { return v[i][tt]; }, ad, head, id, uc,
+                             [&](int i) { return 32 * (L.dh + 2 * i) + L.n; }, 0);
   }
   if (kind < 2) {
     int tok[2];
@@ -191,20 +194,23 @@ constexpr int PROLOGUE_NARROW_TOKENS = 256;
 
 namespace {
 
-template <bool ADAPT>
+template <int RK>
 int launch_prologue(const PrologueArgs& a, const AdapterArgs& ad, hipStream_t s) {
   constexpr int HEADS = HQ + 2 * HKV;
   if (a.tokens >= PROLOGUE_WIDE_TOKENS) {
     const dim3 grid(HEADS * ((a.tokens + WG_TOKENS - 1) / WG_TOKENS));
-    if (a.rope) hipLaunchKernelGGL((qkv_prologue_wide_kernel<true, ADAPT>), grid, dim3(WG_WAVES * WAVE), 0, s, a, ad);
-    else hipLaunchKernelGGL((qkv_prologue_wide_kernel<false, ADAPT>), grid, dim3(WG_WAVES * WAVE), 0, s, a, ad);
+    if (a.rope) hipLaunchKernelGGL((qkv_prologue_wide_kernel<true, RK>), grid, dim3(WG_WAVES * WAVE), 0, s, a, ad);
+    else hipLaunchKernelGGL((qkv_prologue_wide_kernel<false, RK>), grid, dim3(WG_WAVES * WAVE), 0, s, a, ad);
     return launch_status("qkv_prologue_wide_kernel");
   }
   if (a.tokens <= PROLOGUE_NARROW_TOKENS) {
-    hipLaunchKernelGGL((qkv_prologue_kernel<1, ADAPT>), dim3(HEADS * ((a.tokens + 31) / 32)), dim3(4 * WAVE), 0, s, a, ad);
+    const int per_tile = RK ? ad.tile_tokens : 32;
+    hipLaunchKernelGGL((qkv_prologue_kernel<1, RK>), dim3(HEADS * ((a.tokens + per_tile - 1) / per_tile)), dim3(4 * WAVE), 0,
+                       s, a, ad);
     return launch_status("qkv_prologue_kernel");
   }
-  hipLaunchKernelGGL((qkv_prologue_kernel<2, ADAPT>), dim3(HEADS * ((a.tokens + HG_TOKENS - 1) / HG_TOKENS)),
+  const int per_tile = RK ? ad.tile_tokens : HG_TOKENS;
+  hipLaunchKernelGGL((qkv_prologue_kernel<2, RK>), dim3(HEADS * ((a.tokens + per_tile - 1) / per_tile)),
                      dim3(HG_WAVES * WAVE), 0, s, a, ad);
   return launch_status("qkv_prologue_kernel");
 }
@@ -239,25 +245,33 @@ extern "C" int dspark_qkv_prologue(const void* x, const void* wq, const void* wk
   PrologueArgs a{};
   const int rc = check_prologue(a, x, wq, wk, wv, q_norm, k_norm, inv_freq, positions, rope, tokens, hidden, eps, q_out,
                                 k_out, v_out, kv_row_stride);
-  return rc != OK ? rc : launch_prologue<false>(a, AdapterArgs{}, static_cast<hipStream_t>(stream));
+  return rc != OK ? rc : launch_prologue<0>(a, AdapterArgs{}, static_cast<hipStream_t>(stream));
 }
 
 extern "C" int dspark_qkv_prologue_adapted(const void* x, const void* wq, const void* wk, const void* wv,
                                            const void* q_norm, const void* k_norm, const float* inv_freq,
                                            const int64_t* positions, const float* rope, int tokens, int hidden,
-                                           float eps, const int32_t* token_adapter, const void* b, int adapters,
-                                           int rank, const void* u, void* q_out, void* k_out, void* v_out,
-                                           int64_t kv_row_stride, void* stream) {
+                                           float eps, const void* adapter_a, const void* adapter_b, const float* scaling,
+                                           int adapters, int rank, int own_rank, const int32_t* token_adapter,
+                                           const int32_t* tiles, int n_tiles, void* u, void* q_out, void* k_out,
+                                           void* v_out, int64_t kv_row_stride, void* stream) {
   clear_error();
-  DSPARK_REQUIRE(token_adapter && b && u, "null pointer argument");
-  DSPARK_REQUIRE(adapters >= 1 && rank >= 16 && rank % 16 == 0 && rank <= 256,
-                 "need adapters >= 1 and rank a multiple of 16 up to 256");
-  DSPARK_REQUIRE((((uintptr_t)b | (uintptr_t)u) & 15) == 0, "tensors must be 16-byte aligned");
+  DSPARK_REQUIRE(adapter_a && adapter_b && scaling && token_adapter && tiles && u, "null pointer argument");
+  DSPARK_REQUIRE(adapters >= 1 && adapter_rank(rank) && own_rank >= 1 && own_rank <= rank,
+                 "need adapters >= 1, rank 16, 32 or a multiple of 64 up to 256 and own_rank in [1, rank]");
+  DSPARK_REQUIRE(n_tiles >= 1, "n_tiles must be >= 1");
+  DSPARK_REQUIRE((((uintptr_t)adapter_a | (uintptr_t)adapter_b | (uintptr_t)u) & 15) == 0, "tensors must be 16-byte aligned");
   PrologueArgs a{};
-  const int rc = check_prologue(a, x, wq, wk, wv, q_norm, k_norm, inv_freq, positions, rope, tokens, hidden, eps, q_out,
-                                k_out, v_out, kv_row_stride);
-  const AdapterArgs ad{token_adapter, static_cast<const bf16*>(b), static_cast<const bf16*>(u), adapters, rank};
-  return rc != OK ? rc : launch_prologue<true>(a, ad, static_cast<hipStream_t>(stream));
+  int rc = check_prologue(a, x, wq, wk, wv, q_norm, k_norm, inv_freq, positions, rope, tokens, hidden, eps, q_out, k_out,
+                          v_out, kv_row_stride);
+  if (rc != OK) return rc;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  rc = launch_adapter_shrink(ShrinkArgs{a.x, static_cast<const bf16*>(adapter_a), scaling, tiles, static_cast<bf16*>(u),
+                                        tokens, hidden, adapters, rank, own_rank}, n_tiles, s);
+  if (rc != OK) return rc;
+  const AdapterArgs ad{token_adapter, static_cast<const bf16*>(adapter_b), static_cast<const bf16*>(u), adapters, rank,
+                       adapter_tile_tokens(tokens)};
+  return rank == 16 ? launch_prologue<1>(a, ad, s) : rank == 32 ? launch_prologue<2>(a, ad, s) : launch_prologue<4>(a, ad, s);
 }
 
 extern "C" int dspark_rope_table(const float* inv_freq, const int64_t* positions, int tokens, float* table,

@@ -115,9 +115,9 @@ class QKVPrologue:
         into = (q.data_ptr(), outs[0].data_ptr(), outs[1].data_ptr(), KV_HEADS * HEAD_DIM,
                 _native.stream_handle(self.device))
         if adapters is not None and batch.n_tiles:
-            u = adapters.shrink(hidden, batch)
-            _native.call('dspark_qkv_prologue_adapted', *given, batch.token_adapter.data_ptr(), adapters.b.data_ptr(),
-                         adapters.count, adapters.padded_rank, u.data_ptr(), *into)
+            scratch = torch.empty(adapters.scratch(t), dtype=torch.bfloat16, device=self.device)
+            _native.call('dspark_qkv_prologue_adapted', *given, *adapters.pointers, batch.token_adapter.data_ptr(),
+                         batch.tiles.data_ptr(), batch.n_tiles, scratch.data_ptr(), *into)
         else:
             _native.call('dspark_qkv_prologue', *given, *into)
         return q, outs[0], outs[1]
