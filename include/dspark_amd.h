@@ -213,27 +213,30 @@ int dspark_mixed_attn_fwd(const void* q, const void* k, const void* v, const voi
                           int64_t workspace_bytes, void* stream);
 
 /*
- * Attention of query tokens to a prefix that their requests share, for a call of
- * dspark_mixed_attn_fwd behind it on the same stream: FP32 partials of the tokens over
- * resident rows k0 .. k1 - 1 of one slot, all of them visible, left in the partial tiles
- * that the mixed list reserves ahead of the requests' own segments (their records start at
- * the prefix's end, and their request records count both).  No reference counterpart.
- * k_res, v_res and strides as for dspark_verify_attn_fwd.  list (int32, device memory, 16-byte
- * aligned, not validated beyond the bounds given here):
+ * dspark_mixed_attn_fwd over the resident store for a batch in which groups of requests
+ * hold the same committed rows (a prefix): those are attended once per group, in the same
+ * launch.  No reference counterpart.  k_scr / v_scr NULL: the new rows k_new / v_new are
+ * staged already (the scratch's).  The mixed list's records start at the end of their
+ * request's prefix, and its request records count, ahead of the request's own
+ * segments, one partial segment per segment of the prefix.  prefixes (int32, device
+ * memory, 16-byte aligned, not validated beyond the bounds given here):
  *   [0] the number of items, 7 ints unused
- *   [max_items][8] items: slot, k0, k1 (k1 - k0 a multiple of 64), segment number, first token
- *       record, token records (1 to 32), two unused
+ *   [max_items][8] items: slot, k0, k1 (rows of that slot that all of the item's tokens
+ *       see; k1 - k0 a multiple of 64), segment number, first token record, token
+ *       records (1 to 32), two unused
  *   [max_tokens][4] tokens: query row, partial tile of segment 0, the token's place in it
  *       (0 to 7), tiles from one segment to the next
- * Members of the grid (a multiple of 8 workgroups, whose number modulo 8 is their KV head)
- * walk the items; an empty list launches and leaves at once, so that a captured call
- * serves lists to come.  workspace: dspark_attn_workspace_bytes(part_tiles, 0, 1, 32)
- * bytes, the mixed call's.
+ * members workgroups per KV head walk the items; they and the runs are dealt to the CUs in
+ * turns of `turn` (a CU per KV head and column: the CU count / 8).  Lists of any length up
+ * to the bounds, empty ones too, launch alike, so that a captured call serves lists to
+ * come.  workspace: dspark_attn_workspace_bytes(part_tiles, 0, 1, 32) bytes.
  */
-int dspark_prefix_attn_partials(const void* q, int64_t q_rows, const void* k_res, const void* v_res,
-                                int64_t slot_stride, int64_t tok_stride, int64_t head_stride, float scale,
-                                const int32_t* list, int max_items, int max_tokens, int workgroups, int part_tiles,
-                                void* workspace, int64_t workspace_bytes, void* stream);
+int dspark_shared_attn_fwd(const void* q, int64_t q_rows, const void* k_res, const void* v_res, const void* k_new,
+                           const void* v_new, void* k_scr, void* v_scr, int n_req, int64_t slot_stride,
+                           int64_t tok_stride, int64_t head_stride, int max_q, float scale, const int32_t* work,
+                           int n_work, int n_groups, int n_columns, const int32_t* prefixes, int max_items,
+                           int max_tokens, int members, int turn, int part_tiles, void* out, void* workspace,
+                           int64_t workspace_bytes, void* stream);
 
 /*
  * Multi-block DSpark draft attention.  Request r owns blocks

@@ -33,7 +33,8 @@ SIGNATURES = {
                                     _P, _P, _L, _P]),
     'dspark_mixed_attn_fwd': (_I, [_P, _P, _P, _P, _P, _P, _P, _I, _L, _L, _L, _I, _I, _F, _P, _I, _I, _I, _I, _P, _P, _L,
                                    _P]),
-    'dspark_prefix_attn_partials': (_I, [_P, _L, _P, _P, _L, _L, _L, _F, _P, _I, _I, _I, _I, _P, _L, _P]),
+    'dspark_shared_attn_fwd': (_I, [_P, _L, _P, _P, _P, _P, _P, _P, _I, _L, _L, _L, _I, _F, _P, _I, _I, _I, _P, _I, _I, _I, _I,
+                                    _I, _P, _P, _L, _P]),
     'dspark_noalloc_scratch_bytes': (_L, []),
     'dspark_verify_attn_fwd_noalloc': (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _I, _L, _L, _L, _L, _I, _F, _I, _P, _I,
                                             _I, _P, _P]),

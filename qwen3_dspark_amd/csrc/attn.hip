@@ -1844,35 +1844,14 @@ __device__ __forceinline__ void prefill_merge(const VarlenArgs& a, const float* 
   }
 }
 
-// A call whose max_q exceeds DECODE_TOKENS is one launch: first the workgroups that
-// walk the runs, then the prompts'.  With COLUMNS (a mixed plan) those are the listed
-// (record, tile) pairs, in the order of the list, which starts with the longest; else
-// the grid is gridDim.x = 8 x the tiles of max_q wide, its first `decode_rows` rows
-// walk the runs (or fixed chunks), a plane after the other, and one row follows per
-// record: each request is then attended by one of the two forms by its own lengths.
+// The prompt workgroup of list column `column` (COLUMNS), or of record `seg`, tile `t`.
 template <bool VERIFY, bool COLUMNS>
-__global__ __launch_bounds__(PF_WAVES * WAVE, 2) void prefill_attn_kernel(VarlenArgs a, int decode_grid, int decode_rows) {
-  // 1 KiB alignment: tile offsets are XORed into LDS addresses.
-  __shared__ __attribute__((aligned(1024))) unsigned char smem[PF_SMEM];
-  static_assert(PF_SMEM >= VARLEN_SMEM && PF_WAVES * WAVE == 256, "one launch shape for both forms");
-  const int row = blockIdx.y + PF_SEGS_Y * blockIdx.z;
-  const int wid = (int)(blockIdx.x + gridDim.x * (unsigned)row);        // keeps the XCD: gridDim.x is a multiple of 8
-  if (COLUMNS ? wid < decode_grid : row < decode_rows) {
-    if (COLUMNS) {
-      varlen_workgroup<VERIFY, true, RECORDS>(a, smem, wid, decode_grid, 0);
-    } else {
-      const int plane = wid / decode_grid;
-      if (plane < a.planes) varlen_workgroup<VERIFY, true, PLANES>(a, smem, wid - plane * decode_grid, decode_grid, plane);
-    }
-    return;
-  }
+__device__ __forceinline__ void prefill_workgroup(const VarlenArgs& a, unsigned char* smem, int column, int seg, int t) {
   const int g = blockIdx.x & 7;
-  int t = (gridDim.x >> 3) - 1 - (blockIdx.x >> 3);
-  int seg = row - decode_rows;
   if (COLUMNS) {
-    const int32_t* column = a.columns + 2 * ((wid - decode_grid) >> 3);
-    seg = min(__builtin_amdgcn_readfirstlane(column[0]), a.n_work) - 1;
-    t = max(__builtin_amdgcn_readfirstlane(column[1]), 0);
+    const int32_t* pair = a.columns + 2 * column;
+    seg = min(__builtin_amdgcn_readfirstlane(pair[0]), a.n_work) - 1;
+    t = max(__builtin_amdgcn_readfirstlane(pair[1]), 0);
   } else if (a.work) {
     seg = a.n_work - 1 - seg;        // a plan puts its prompts after the runs, longest last
   }
@@ -2082,6 +2061,32 @@ __global__ __launch_bounds__(PF_WAVES * WAVE, 2) void prefill_attn_kernel(Varlen
   }
 }
 
+// A call whose max_q exceeds DECODE_TOKENS is one launch: first the workgroups that
+// walk the runs, then the prompts'.  With COLUMNS (a mixed plan) those are the listed
+// (record, tile) pairs, in the order of the list, which starts with the longest; else
+// the grid is gridDim.x = 8 x the tiles of max_q wide, its first `decode_rows` rows
+// walk the runs (or fixed chunks), a plane after the other, and one row follows per
+// record: each request is then attended by one of the two forms by its own lengths.
+template <bool VERIFY, bool COLUMNS>
+__global__ __launch_bounds__(PF_WAVES * WAVE, 2) void prefill_attn_kernel(VarlenArgs a, int decode_grid, int decode_rows) {
+  // 1 KiB alignment: tile offsets are XORed into LDS addresses.
+  __shared__ __attribute__((aligned(1024))) unsigned char smem[PF_SMEM];
+  static_assert(PF_SMEM >= VARLEN_SMEM && PF_WAVES * WAVE == 256, "one launch shape for both forms");
+  const int row = blockIdx.y + PF_SEGS_Y * blockIdx.z;
+  const int wid = (int)(blockIdx.x + gridDim.x * (unsigned)row);        // keeps the XCD: gridDim.x is a multiple of 8
+  if (COLUMNS ? wid < decode_grid : row < decode_rows) {
+    if (COLUMNS) {
+      varlen_workgroup<VERIFY, true, RECORDS>(a, smem, wid, decode_grid, 0);
+    } else {
+      const int plane = wid / decode_grid;
+      if (plane < a.planes) varlen_workgroup<VERIFY, true, PLANES>(a, smem, wid - plane * decode_grid, decode_grid, plane);
+    }
+    return;
+  }
+  prefill_workgroup<VERIFY, COLUMNS>(a, smem, (wid - decode_grid) >> 3, row - decode_rows,
+                                     (int)(gridDim.x >> 3) - 1 - (int)(blockIdx.x >> 3));
+}
+
 // ---------------------------------------------------------------------------
 // A prefix that many requests of a verification batch share (the same committed rows, of
 // which each keeps a copy): attended once for all of them
@@ -2110,8 +2115,60 @@ struct PrefixArgs {
   float scale_log2;
 };
 
-__global__ __launch_bounds__(PF_WAVES * WAVE, 2) void prefix_attn_kernel(PrefixArgs a) {
-  __shared__ __attribute__((aligned(1024))) unsigned char smem[PF_SMEM];
+// Probabilities of a tile of raw scores x against m_use, rounded to bf16 for PV; the
+// denominator sums them unrounded.  One operand, as in the 8-token workgroups that attend
+// the requests' own keys: ONEOP.
+__device__ __forceinline__ void prefix_probs(PairState& st, const f32x16& x, float m_use, float scale_log2, bf16x8 (&p)[2]) {
+  float ps[2] = {0.f, 0.f};
+  #pragma unroll
+  for (int r = 0; r < 16; r += 2) {
+    float e[2];
+    #pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      e[i] = fast_exp2(__builtin_fmaf(x[r + i], scale_log2, -m_use));
+      ps[i] += e[i];
+    }
+    p[r >> 3][r & 7] = (bf16)e[0];
+    p[r >> 3][(r & 7) + 1] = (bf16)e[1];
+  }
+  st.l += ps[0] + ps[1];
+}
+
+// prefill_full_tile with one operand: the scores of the next tile beside this one's maximum
+// and exponentials, then PV.
+__device__ __forceinline__ f32x16 prefix_tile(PairState& st, const bf16x8 (&qf)[8], const f32x16& x, uint32_t ka,
+                                              uint32_t va, float scale_log2) {
+  bf16x8 kf[8], vt[2][4];
+  prefill_k(kf, ka);
+  __builtin_amdgcn_sched_barrier(0);
+  const float m_use = prefill_max(st, x, scale_log2);
+  #pragma unroll
+  for (int t = 0; t < 2; ++t)
+    #pragma unroll
+    for (int D = 0; D < 4; ++D) vt[t][D] = prefill_v(va, t, D);
+  bf16x8 p[2];
+  f32x16 nx = prefill_scores<0, 8>(qf, kf);
+  prefix_probs(st, x, m_use, scale_log2, p);
+  #pragma unroll
+  for (int t = 0; t < 2; ++t)
+    #pragma unroll
+    for (int D = 0; D < 4; ++D) st.o[D] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vt[t][D], p[t], st.o[D], 0, 0, 0);
+  #pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+    __builtin_amdgcn_sched_group_barrier(0x002, 8, 0);
+  }
+  #pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+    __builtin_amdgcn_sched_group_barrier(0x002, 6, 0);
+  }
+  __builtin_amdgcn_sched_group_barrier(0x008, 4, 0);
+  return nx;
+}
+
+// The items `member`, `member` + members, .. of the list.
+__device__ __forceinline__ void prefix_workgroup(const PrefixArgs& a, unsigned char* smem, int member, int members) {
   const int g = blockIdx.x & 7;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
@@ -2126,7 +2183,7 @@ __global__ __launch_bounds__(PF_WAVES * WAVE, 2) void prefix_attn_kernel(PrefixA
   const int32_t* items = a.list + WORK_INTS;
   const int32_t* tokens = items + WORK_INTS * a.max_items;
   const int n_items = min(ld_const(a.list), a.max_items);
-  for (int it = blockIdx.x >> 3; it < n_items; it += gridDim.x >> 3) {
+  for (int it = member; it < n_items; it += members) {
     const int32_t* w = items + WORK_INTS * it;
     const int slot = ld_const(w, 0), k0 = ld_const(w, 1), k1 = ld_const(w, 2), seg = ld_const(w, 3);
     const int first = ld_const(w, 4), n_tok = min(ld_const(w, 5), min(PF_TOKENS, a.max_tokens - first));
@@ -2195,13 +2252,13 @@ __global__ __launch_bounds__(PF_WAVES * WAVE, 2) void prefix_attn_kernel(PrefixA
     if (kg_count == 2) {
       for (; s + 1 < n_steps; s += 2) {
         enter(s);
-        const f32x16 y = prefill_full_tile(st, qf, x, k_at(s + 1), v_at(s), a.scale_log2);
+        const f32x16 y = prefix_tile(st, qf, x, k_at(s + 1), v_at(s), a.scale_log2);
         enter(s + 1);
-        x = prefill_full_tile(st, qf, y, k_at(s + 2), v_at(s + 1), a.scale_log2);
+        x = prefix_tile(st, qf, y, k_at(s + 2), v_at(s + 1), a.scale_log2);
       }
       if (s < n_steps) {
         enter(s);
-        x = prefill_full_tile(st, qf, x, k_at(s + 1), v_at(s), a.scale_log2);
+        x = prefix_tile(st, qf, x, k_at(s + 1), v_at(s), a.scale_log2);
         ++s;
       }
     }
@@ -2209,15 +2266,14 @@ __global__ __launch_bounds__(PF_WAVES * WAVE, 2) void prefix_attn_kernel(PrefixA
       enter(s);
       if (turn(s)) {
         const float m_use = prefill_max(st, x, a.scale_log2);
-        bf16x8 ph[2], pl[2];
-        prefill_probs(st, x, m_use, a.scale_log2, ph, pl);
+        bf16x8 p[2];
+        prefix_probs(st, x, m_use, a.scale_log2, p);
         #pragma unroll
         for (int u = 0; u < 2; ++u)
           #pragma unroll
           for (int D = 0; D < 4; ++D) {
             const bf16x8 vt = prefill_v(v_at(s), u, D);
-            st.o[D] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vt, ph[u], st.o[D], 0, 0, 0);
-            st.o[D] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vt, pl[u], st.o[D], 0, 0, 0);
+            st.o[D] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vt, p[u], st.o[D], 0, 0, 0);
           }
       }
       if (turn(s + 1)) x = ahead(s + 1);
@@ -2271,6 +2327,27 @@ __global__ __launch_bounds__(PF_WAVES * WAVE, 2) void prefix_attn_kernel(PrefixA
     }
     __syncthreads();   // the next item's stages reuse the merge space
   }
+}
+
+// One launch for all parts of a batch: `members` x 8 workgroups walk the prefix items,
+// `runs` x 8 the runs of the requests' own keys, then one follows per (prompt column, KV
+// head).  The first two are dealt in turns of `turn` columns, a CU's worth each, so that a CU
+// has one of either: the prefix's are bound by the matrix units, the runs by memory.
+template <bool COLUMNS>
+__global__ __launch_bounds__(PF_WAVES * WAVE, 2) void shared_attn_kernel(VarlenArgs a, PrefixArgs p, int members, int runs,
+                                                                         int turn) {
+  __shared__ __attribute__((aligned(1024))) unsigned char smem[PF_SMEM];
+  const int c = blockIdx.x >> 3;
+  if (c >= members + runs) {
+    if constexpr (COLUMNS) prefill_workgroup<true, true>(a, smem, c - members - runs, 0, 0);
+    return;
+  }
+  const int both = min(members, runs) / turn * turn;             // of either, in turns
+  const int round = c / (2 * turn), at = c % (2 * turn);
+  const bool prefix = c < 2 * both ? at < turn : c - 2 * both < members - both;
+  const int i = c < 2 * both ? round * turn + at % turn : prefix ? c - both : c - members;
+  if (prefix) prefix_workgroup(p, smem, i, members);
+  else varlen_workgroup<true, COLUMNS, RECORDS>(a, smem, 8 * i + (blockIdx.x & 7), 8 * runs, 0);
 }
 
 // ---------------------------------------------------------------------------
@@ -2625,32 +2702,68 @@ extern "C" int dspark_mixed_attn_fwd(const void* q, const void* k, const void* v
   return launch_merge(m, n_req, tiles, s);
 }
 
-extern "C" int dspark_prefix_attn_partials(const void* q, int64_t q_rows, const void* k_res, const void* v_res,
-                                           int64_t slot_stride, int64_t tok_stride, int64_t head_stride, float scale,
-                                           const int32_t* list, int max_items, int max_tokens, int workgroups,
-                                           int part_tiles, void* workspace, int64_t workspace_bytes_, void* stream) {
+extern "C" int dspark_shared_attn_fwd(const void* q, int64_t q_rows, const void* k_res, const void* v_res, const void* k_new,
+                                      const void* v_new, void* k_scr, void* v_scr, int n_req, int64_t slot_stride,
+                                      int64_t tok_stride, int64_t head_stride, int max_q, float scale,
+                                      const int32_t* work, int n_work, int n_groups, int n_columns,
+                                      const int32_t* prefixes, int max_items, int max_tokens, int members, int turn,
+                                      int part_tiles, void* out, void* workspace, int64_t workspace_bytes_,
+                                      void* stream) {
   clear_error();
-  DSPARK_REQUIRE(q && k_res && v_res && list && workspace, "null pointer argument");
-  DSPARK_REQUIRE(aligned16(q) && aligned16(k_res) && aligned16(v_res) && aligned16(list) && aligned16(workspace),
-                 "Q/K/V, the list and the workspace must be 16-byte aligned");
+  DSPARK_REQUIRE(q && k_res && v_res && k_new && v_new && work && prefixes && out && workspace, "null pointer argument");
+  DSPARK_REQUIRE((k_scr != nullptr) == (v_scr != nullptr), "k_scr and v_scr go together");
+  DSPARK_REQUIRE(aligned16(q) && aligned16(k_res) && aligned16(v_res) && aligned16(k_new) && aligned16(v_new) &&
+                 aligned16(k_scr) && aligned16(v_scr) && aligned16(prefixes) && aligned16(out) && aligned16(workspace),
+                 "Q/K/V/out, the prefix list and the workspace must be 16-byte aligned");
   DSPARK_REQUIRE(slot_stride >= 0 && tok_stride >= HD && tok_stride % 8 == 0 && head_stride >= HD && head_stride % 8 == 0,
                  "resident strides must be multiples of 8 elements (token/head strides >= 128)");
   DSPARK_REQUIRE(q_rows >= 1 && q_rows <= 0x7fffffffLL, "q_rows must be in [1, 2^31)");
+  DSPARK_REQUIRE(max_q >= 1, "max_q must be >= 1");
+  DSPARK_REQUIRE(n_work >= 1 && n_groups >= 8 && n_groups <= (1 << 24) && n_groups % 8 == 0 && n_columns >= 0 &&
+                 n_columns <= (1 << 24), "need n_work >= 1, n_groups a multiple of 8 in [8, 2^24] and n_columns in [0, 2^24]");
   DSPARK_REQUIRE(max_items >= 1 && max_tokens >= 1 && max_items <= (1 << 24) && max_tokens <= (1 << 26),
                  "need max_items in [1, 2^24] and max_tokens in [1, 2^26]");
-  DSPARK_REQUIRE(workgroups >= 8 && workgroups % 8 == 0 && workgroups <= (1 << 20), "workgroups must be a multiple of 8 in [8, 2^20]");
-  DSPARK_REQUIRE(scale > 0.f && scale < 1e30f, "scale must be positive and finite");
+  DSPARK_REQUIRE(members >= 1 && members <= (1 << 16) && turn >= 1 && turn <= (1 << 16), "members and turn must be in [1, 2^16]");
+  const int tiles = (max_q + 7) / 8;
+  int rc = check_shape(n_req, 0, tiles, 32, scale);
+  if (rc != OK) return rc;
   DSPARK_REQUIRE(part_tiles >= 1, "part_tiles must be >= 1");
   const int64_t need = dspark_attn_workspace_bytes(part_tiles, 0, 1, 32);
   DSPARK_REQUIRE(workspace_bytes_ >= need, "workspace too small: %lld < %lld bytes", (long long)workspace_bytes_,
                  (long long)need);
-  PrefixArgs a{static_cast<const bf16*>(q), static_cast<const bf16*>(k_res), static_cast<const bf16*>(v_res), slot_stride,
-               tok_stride, head_stride, list, static_cast<float*>(workspace), nullptr, max_items, max_tokens, part_tiles,
-               (int)q_rows, scale * LOG2E};
+  VarlenArgs a{};
+  a.q = static_cast<const bf16*>(q);
+  a.k_a = static_cast<const bf16*>(k_res);
+  a.v_a = static_cast<const bf16*>(v_res);
+  a.k_b = static_cast<const bf16*>(k_new);
+  a.v_b = static_cast<const bf16*>(v_new);
+  a.stage_k = static_cast<bf16*>(k_scr);
+  a.stage_v = static_cast<bf16*>(v_scr);
+  a.slot_stride = slot_stride;
+  a.a_tok_stride = tok_stride;
+  a.a_head_stride = head_stride;
+  a.work = work;
+  a.out = static_cast<bf16*>(out);
+  a.part_o = static_cast<float*>(workspace);
   a.part_ml = a.part_o + (int64_t)part_tiles * HKV * 16 * HD;
-  hipLaunchKernelGGL(prefix_attn_kernel, dim3((unsigned)workgroups), dim3(PF_WAVES * WAVE), 0,
-                     static_cast<hipStream_t>(stream), a);
-  return launch_status("prefix_attn_kernel");
+  a.n_req = n_req;
+  a.n_work = n_work;
+  a.n_groups = n_groups;
+  a.causal = 1;
+  a.tmax = 0;
+  a.scale_log2 = scale * LOG2E;
+  const int32_t* requests = work + WORK_INTS * n_work + n_groups + 1;
+  a.columns = requests + REQ_INTS * n_req;
+  const PrefixArgs p{a.q, a.k_a, a.v_a, slot_stride, tok_stride, head_stride, prefixes, a.part_o, a.part_ml, max_items,
+                     max_tokens, part_tiles, (int)q_rows, a.scale_log2};
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  const dim3 grid((unsigned)(members + n_groups + n_columns) * HKV);
+  hipLaunchKernelGGL((n_columns ? shared_attn_kernel<true> : shared_attn_kernel<false>), grid, dim3(PF_WAVES * WAVE), 0, s, a,
+                     p, members, n_groups, turn);
+  rc = launch_status("shared_attn_kernel");
+  if (rc != OK) return rc;
+  MergeArgs m{requests, nullptr, nullptr, nullptr, nullptr, a.part_o, a.part_ml, a.out, n_req, 0, 0, 0};
+  return launch_merge(m, n_req, tiles, s);
 }
 
 // ---------------------------------------------------------------------------

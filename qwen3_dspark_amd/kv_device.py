@@ -25,7 +25,7 @@ import torch
 from . import _native
 from ._device import KV_PAIR_SKEW, cu_count, kv_pair, require_gfx950, upload
 from .kernels import HEAD_DIM, KV_HEADS, SCALE
-from .shared_prefix import mixed_part_ints, shared_bytes, shared_capacity, shared_ints, shared_plan
+from .shared_prefix import mixed_part_ints, prefix_columns, shared_bytes, shared_capacity, shared_ints, shared_plan
 from .schedule import (DECODE_TOKENS, PART_TILE_BYTES, REQ_INTS, TILED_TOKENS, WORK_INTS, XCDS, check_chunk,
                        mixed_capacity, mixed_ints, mixed_plan, run_count, segment_plan, varlen_list_bound)
 
@@ -291,14 +291,18 @@ class HipKVDevice:
         C = self.capacity
         k, v, sk, sv = self.layer_pointers[layer]
         if self.shared:
-            c = self.shared_counts(shape)
-            capacity, counts = c, (c.run_records + c.prompt_records, c.runs, c.requests, c.columns, c.tiles)
-            _native.call('dspark_prefix_attn_partials', query, shape.query_tokens, k, v, KV_HEADS * C * HEAD_DIM, HEAD_DIM,
-                         C * HEAD_DIM, SCALE, ws.work.data_ptr() + 4 * mixed_part_ints(c), c.items, c.tokens,
-                         8 * c.runs, c.tiles, ws.attn.data_ptr(), ws.attn.numel(),
-                         _native.stream_handle(self.device))
-        else:
-            capacity, counts = self.list_counts(ws, shape)
+            if ws.counts is None:
+                c, per_cu = self.shared_counts(shape), max(1, cu_count(self.device) // 8)
+                ws.counts = (shape.query_tokens, c.requests, shape.maximum_query_length, c.run_records + c.prompt_records,
+                             c.runs, c.columns, ws.work.data_ptr() + 4 * mixed_part_ints(c), c.items, c.tokens,
+                             prefix_columns(per_cu), per_cu, c.tiles)
+            rows, requests, longest, n_work, runs, columns, *prefixes = ws.counts
+            new = (sk, sv, None, None) if keys is None else (keys, values, sk, sv)
+            _native.call('dspark_shared_attn_fwd', query, rows, k, v, *new, requests, KV_HEADS * C * HEAD_DIM, HEAD_DIM,
+                         C * HEAD_DIM, longest, SCALE, ws.work.data_ptr(), n_work, runs, columns, *prefixes, out,
+                         ws.attn.data_ptr(), ws.attn.numel(), _native.stream_handle(self.device))
+            return
+        capacity, counts = self.list_counts(ws, shape)
         if capacity is not None:
             check_chunk(self.chunk)
             n_work, runs, requests, columns, tiles = counts

@@ -25,8 +25,22 @@ from .schedule import (DECODE_TOKENS, PART_TILE_BYTES, PROMPT_TOKENS, REQ_INTS, 
                        XCDS, _balanced_runs, _prompt_columns, prompt_segments, run_count, run_shares)
 
 PREFIX_TILE = 64              # prefixes end, and are cut, at multiples of this many keys (a ring stage)
-MIN_SHARED = 64               # fewest common rows that form a group
-MIN_PREFIX_SEGMENT = 256      # fewest keys of a prefix segment
+# Fewest key rows that a group must save to be one: sharing takes partials and a second part.
+# Shared / each request its own copy, us a call: 2 requests of 7 tokens over 1,000 rows
+# 13.1 / 11.1, 4 over 1,000 14.0 / 12.2, 2 over 4,000 16.3 / 16.7, 16 over 2,000 19.4 / 28.6, 64 over
+# 8,192 56 / 353.
+MIN_SAVED = 4096
+# Prefix workgroups per CU, in the kernel's grid.  Their segments are counted for one: beside
+# them on a CU is a run of the requests' own keys, which memory bounds.  Segments for one / two
+# per CU, us a call: 64 requests of 1 to 8 tokens over 8,192 rows and up to 1,024 own 57 / 61, 8
+# of 7 over 16,384 27 / 38, 64 of 8 over 16,384 112 / 107, 12 prompts over 6,000 162 / 166.
+PREFIX_PER_CU = 2
+MIN_PREFIX_SEGMENT = 128      # fewest keys of a prefix segment
+MAX_PREFIX_SEGMENTS = 32
+# A segment's fixed work (its start, partials and their merge), in keys.  With 192 and 400: 6
+# prompts of up to 100 tokens over 2,000 rows 27 and 22 us, 3 of 400 over 3,000 65 and 61, 64 requests
+# over 8,192 56 and 57.
+PREFIX_SEGMENT_COST = 400
 PREFIX_TILES = 1024           # partial tiles that prefix segments may take (more where one segment each needs it)
 TOKEN_INTS = 4
 
@@ -76,7 +90,7 @@ def shared_groups(lineages, contexts, slots):
             best = max(range(2, len(members) + 1), key=lambda n: (n - 1) * (span[members[n - 1]] // PREFIX_TILE))
             chosen = members[:best]
             rows = span[chosen[-1]] // PREFIX_TILE * PREFIX_TILE
-            if rows < MIN_SHARED:
+            if rows == 0 or (best - 1) * rows < MIN_SAVED:
                 break
             groups.append(Group(sorted(chosen), rows, slots[min(chosen)]))
             members = members[best:]
@@ -98,7 +112,7 @@ def shared_capacity(n_req, query_tokens, max_q, n_cu):
     own = width + n_req + slots + (PROMPT_TOKENS // DECODE_TOKENS * slots if prompts else 0)
     tiles = query_tokens // PROMPT_TOKENS + n_req                      # 32-token tiles at most
     return SharedCapacity(n_req + slots - 1, n_req + slots - 1 if prompts else 0, slots, n_req,
-                          max(slots, tiles) if prompts else 0, own + prefix, prefix, 2 * slots + tiles, query_tokens)
+                          max(slots, tiles) if prompts else 0, own + prefix, prefix, prefix + tiles, query_tokens)
 
 
 def mixed_part_ints(c):
@@ -116,11 +130,17 @@ def shared_bytes(c):
     return PART_TILE_BYTES * c.tiles
 
 
-def prefix_segments(tokens, rows, columns, room):
-    """Segments of a group's prefix: about `columns` (token tile, segment) items per KV
-    head, of at least MIN_PREFIX_SEGMENT keys, `room` at most."""
-    tiles = -(-tokens // PROMPT_TOKENS)
-    return max(1, min(columns // tiles, rows // MIN_PREFIX_SEGMENT, room))
+def prefix_columns(per_cu):
+    """Prefix workgroups per KV head, for `per_cu` CUs per KV head."""
+    return PREFIX_PER_CU * per_cu
+
+
+def prefix_segments(tiles, rows, columns, room):
+    """Segments of a group's prefix, for `tiles` token tiles per segment on `columns` workgroup
+    slots per KV head: of those that keep MIN_PREFIX_SEGMENT keys each and fit `room`
+    partials, the number whose rounds of slots take the least time."""
+    most = max(1, min(rows // MIN_PREFIX_SEGMENT, MAX_PREFIX_SEGMENTS, room))
+    return min(range(1, most + 1), key=lambda p: -(-tiles * p // columns) * (rows / p + PREFIX_SEGMENT_COST))
 
 
 def shared_plan(query_lengths, key_lengths, starts, groups, n_cu, capacity, *, xcd_speed=None, slot_balance=True):
@@ -137,7 +157,7 @@ def shared_plan(query_lengths, key_lengths, starts, groups, n_cu, capacity, *, x
     width = [_width(q) for q in query_lengths]
 
     # the prefixes' segments: the groups share the columns by their work, and the room for partials
-    per_head = max(XCDS, RESIDENT_PER_CU * n_cu // 8 // XCDS * XCDS)
+    per_head = max(1, n_cu // 8)
     work = [sum(query_lengths[r] for r in group.members) * group.length for group in groups]
     least = sum(width[r] for group in groups for r in group.members)
     parts, prefix_parts, items, tokens = [], [0] * n, [], []
@@ -145,7 +165,7 @@ def shared_plan(query_lengths, key_lengths, starts, groups, n_cu, capacity, *, x
         wide = sum(width[r] for r in group.members)
         share = max(1, per_head * cost // sum(work))
         room = max(1, c.prefix_tiles * wide // least // wide)
-        p = prefix_segments(sum(query_lengths[r] for r in group.members), group.length, share, room)
+        p = prefix_segments(-(-sum(query_lengths[r] for r in group.members) // PROMPT_TOKENS), group.length, share, room)
         parts.append(p)
         for r in group.members:
             prefix_parts[r] = p

@@ -12,6 +12,12 @@ pytestmark = pytest.mark.gpu
 DEV = torch.device('cuda:0')
 
 
+@pytest.fixture(autouse=True)
+def groups_of_any_size(monkeypatch):
+    from qwen3_dspark_amd import shared_prefix
+    monkeypatch.setattr(shared_prefix, 'MIN_SAVED', 0)
+
+
 def build(families, *, layers=1, capacity=6144, rows=512, seed=0, extra=0, shared=True, shuffle=True):
     """A store and its requests: families [(prefix rows, [own rows, ..])]; the first of a family
     is the one that the others copy."""
@@ -187,6 +193,18 @@ def test_sharing_through_steps_and_departures():
     kv = randn_bf16(gen, 2, 2, 800, 8, 128).to(DEV)
     store.load_prefix(e, kv[0], kv[1])
     round_([e, b, c, d])
+
+
+def test_small_groups_are_attended_request_by_request(monkeypatch):
+    from qwen3_dspark_amd.persistent_kv import Bucket
+    monkeypatch.undo()
+    store, handles, gen = build([(1000, [3, 40])])
+    bucket = Bucket((7, 2), (2000,) * 2, 'round')
+    store.register_bucket(bucket)
+    q, nk, nv = (randn_bf16(gen, 9, h, 128).to(DEV) for h in (16, 8, 8))
+    want = expected(store, handles, (7, 2), q, nk, nv)
+    tx = store.begin(handles, bucket)
+    check(store.attend(tx, 0, q, keys=nk, values=nv), want)
 
 
 def test_far_slots():

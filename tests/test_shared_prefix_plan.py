@@ -7,6 +7,7 @@ import pytest
 import torch
 
 from kv_fake import store
+from qwen3_dspark_amd import shared_prefix
 from qwen3_dspark_amd.schedule import REQ_INTS, WORK_INTS
 from qwen3_dspark_amd.shared_prefix import (PREFIX_TILE, common_rows, inherited, mixed_part_ints, shared_capacity,
                                             shared_groups, shared_ints, shared_plan)
@@ -22,6 +23,11 @@ def test_lineages():
     assert [common_rows(*x) for x in ((a, b), (b, d), (a, d), (d, inherited(a, 300, 7)), (a, ((9, None),)))] == \
         [1000, 1500, 1000, 300, 0]
     assert common_rows(a, a) is None
+
+
+@pytest.fixture(autouse=True)
+def groups_of_any_size(monkeypatch):
+    monkeypatch.setattr(shared_prefix, 'MIN_SAVED', 0)
 
 
 def rows_of(lineage, length):
@@ -154,6 +160,15 @@ def test_members_that_would_shorten_a_group_stay_out():
     assert [(g.members, g.length, g.slot) for g in groups] == [([0, 1, 2], 3968, 4), ([3, 4], 64, 1)]
     assert shared_groups(lineages[3:], [63, 400], [1, 0]) == []
     assert shared_groups([a], [5000], [0]) == []
+
+
+def test_groups_that_would_save_little_are_none(monkeypatch):
+    monkeypatch.undo()
+    a = ((0, None),)
+    lineages = [a, *(inherited(a, 2048, r) for r in range(1, 4))]
+    assert shared_groups(lineages[:2], [2048] * 2, [0, 1]) == []
+    assert [g.length for g in shared_groups(lineages[:3], [2048] * 3, [0, 1, 2])] == [2048]
+    assert [g.length for g in shared_groups(lineages, [2048, 1500, 1500, 1500], [0, 1, 2, 3])] == [1472]
 
 
 def test_share_prefix_in_the_store():
