@@ -106,11 +106,33 @@ def test_proposals_and_texts(counts, history):
     check(b.call(), b.expected(), torch.float32)
 
 
+@pytest.mark.parametrize('dtype,out', [(torch.bfloat16, None), (torch.bfloat16, torch.float32), (torch.float32, None)])
+@pytest.mark.parametrize('mask', [False, True])
+@pytest.mark.parametrize('vocab,pad', [(700, 3), (8192, 0), (17001, 5)])
+def test_texts_that_are_long_for_their_rows(vocab, pad, mask, dtype, out):
+    b = Batch(vocab, [0, 1], 12000, dtype, seed=pad, pad=pad, mask=mask, out=out,
+              hist_dtype=torch.int32 if mask else torch.long)
+    assert sum(b.lengths) > 2048 * 3
+    if mask:
+        b.allowed[1] = False
+    o = None if out is None else torch.empty(b.logits.shape, dtype=out, device=DEV)
+    check(b.call(out=o), b.expected(), b.out_dtype)
+
+
+def test_many_requests():
+    """More than a launch's arguments hold: the layout is uploaded."""
+    b = Batch(300, [1] * 129 + [0, 3], 20, torch.float32, seed=9)
+    check(b.call(), b.expected(), torch.float32)
+
+
 def test_in_place_gives_the_same_bits():
     b = Batch(8200, [3, 0, 5], 400, torch.bfloat16)
     want = b.call()
     got = b.call(out=b.logits)
     assert got.data_ptr() == b.logits.data_ptr() and torch.equal(got, want)
+    c = Batch(8200, [3], 400, torch.float32, mask=False, pad=3)
+    want = c.call()
+    assert torch.equal(c.call(out=c.logits), want)
 
 
 def test_rows_that_allow_nothing_and_values_that_are_none():
