@@ -60,7 +60,7 @@ __global__ __launch_bounds__(4 * TG * WAVE) void qkv_prologue_kernel(PrologueArg
   const int slot = blockIdx.x >> 3;
   const int head = xcd + 8 * (slot / tiles);
   const int t0 = (slot % tiles) * per_tile;
-  const int end = min(t0 + per_tile, a.tokens);
+  const int end = RK ? min(t0 + per_tile, a.tokens) : a.tokens;
   const int kind = head < HQ ? 0 : (head < HQ + HKV ? 1 : 2);       // workgroup-uniform
   const int hh = kind == 0 ? head : (kind == 1 ? head - HQ : head - HQ - HKV);
   const bf16* w = (kind == 0 ? a.wq : (kind == 1 ? a.wk : a.wv)) + (size_t)hh * HD * a.hidden;
