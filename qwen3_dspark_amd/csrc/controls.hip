@@ -362,7 +362,8 @@ int launch_controls(const ControlArgs& a, int64_t text_tokens, int64_t rows, hip
 
 extern "C" int dspark_logit_controls(const void* logits, int dtype, int64_t row_stride, int vocab,
                                      const int32_t* layout, int host_layout, int n_req, int64_t rows,
-                                     int64_t text_tokens, const void* history, int history_bytes, int64_t history_stride, const int64_t* tokens,
+                                     int64_t text_tokens, const void* history, int history_bytes,
+                                     int64_t history_stride, const int64_t* tokens,
                                      const double* penalties, const int32_t* bias_start, const int32_t* bias_token,
                                      const double* bias_value, const int32_t* allowed, int64_t allowed_stride, float fill,
                                      void* out, int out_dtype, int64_t out_stride, void* stream) {
@@ -370,7 +371,8 @@ extern "C" int dspark_logit_controls(const void* logits, int dtype, int64_t row_
   DSPARK_REQUIRE(logits && layout && history && penalties && bias_start && out, "null pointer argument");
   DSPARK_REQUIRE(n_req >= 1 && n_req <= 65535, "n_req must be in [1, 65535] (got %d)", n_req);
   DSPARK_REQUIRE(rows >= 1 && text_tokens >= 0, "need rows >= 1 and text_tokens >= 0");
-  DSPARK_REQUIRE(vocab >= 1 && row_stride >= vocab && out_stride >= vocab, "need vocab >= 1 and row strides of at least vocab");
+  DSPARK_REQUIRE(vocab >= 1 && vocab <= (1 << 30) && row_stride >= vocab && out_stride >= vocab,
+                 "need vocab in [1, 2^30] and row strides of at least vocab");
   DSPARK_REQUIRE(dtype == 0 || dtype == 1, "dtype must be 0 (bf16) or 1 (fp32)");
   DSPARK_REQUIRE(out_dtype == 1 || out_dtype == dtype, "out_dtype must be the logits' or 1 (fp32)");
   DSPARK_REQUIRE(history_bytes == 4 || history_bytes == 8, "history must be int32 or int64");

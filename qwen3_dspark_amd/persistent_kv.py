@@ -320,6 +320,7 @@ class PersistentTargetKV:
         self._staged = set()
         self._tx_rows = 0
         self._rope = {}                  # theta -> rotary table of the open transaction's rows
+        self._groups = ()                # its groups of requests with common rows
         self._receipt = None             # (ExternalWrite, completion event) while one is live
 
     # -- phase ------------------------------------------------------------
@@ -628,14 +629,17 @@ class PersistentTargetKV:
             raise ValueError('Actual context exceeds declared bucket applicability')
         if sum(contexts) + sum(query_lengths) >= 2 ** 31:
             raise ValueError('Varlen cumulative lengths exceed int32')
-        shared = ({'groups': shared_groups([self._ledger.lineage(i) for i in slots], contexts, slots)}
-                  if self.shared_prefixes else {})
+        groups, shared = (), {}
+        if self.shared_prefixes:
+            groups = shared_groups([self._ledger.lineage(i) for i in slots], contexts, slots)
+            shared = dict(groups=groups)
         self.kv_device.build_metadata(self._workspaces[bucket], bucket, slots, contexts, query_lengths, **shared)
         self._transactions += 1
         tx = Transaction(self._transactions, handles, contexts, bucket, query_lengths)
         self._phase, self._tx, self._tx_generation = nxt, tx, self._ledger.generation
         self._staged, self._tx_rows, self._receipt = set(), sum(query_lengths), None
         self._rope = {}                  # theta -> rotary table of this transaction's rows
+        self._groups = groups
         return tx
 
     @torch.no_grad()
@@ -788,6 +792,7 @@ class PersistentTargetKV:
             bucket_workspace_bytes=ws.nbytes(),
             workspace_is_shared=shared,
             shared_arena_allocated_bytes=self.workspace_bytes(self._arena[0]) if shared else 0)
-        counters.update(fused_attention_key_rows_per_layer=keys, bucket_source=bucket.source,
+        saved = sum((len(group.members) - 1) * group.length for group in self._groups)      # attended once per group
+        counters.update(fused_attention_key_rows_per_layer=keys - saved, bucket_source=bucket.source,
                         capture_or_replay_verified=False)
         return counters

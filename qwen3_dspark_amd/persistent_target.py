@@ -261,7 +261,7 @@ class PersistentQwenTarget:
 
     def __init__(self, model, layer_ids=(), *, slots, context_capacity, max_query_tokens, test_kernel=None,
                  native_backend=None, graph_backend=None, max_buckets=32, workspace_byte_budget=256 * 1024 ** 2,
-                 max_graph_buckets=0, graph_byte_budget=0, chunk=DEFAULT_CHUNK):
+                 max_graph_buckets=0, graph_byte_budget=0, chunk=DEFAULT_CHUNK, shared_prefixes=False):
         cfg = model.config
         if (cfg.model_type != 'qwen3' or getattr(cfg, 'use_sliding_window', False)
                 or any(kind != 'full_attention' for kind in cfg.layer_types)
@@ -291,7 +291,8 @@ class PersistentQwenTarget:
         old_backend = cfg._attn_implementation
         store = PersistentTargetKV(layers=cfg.num_hidden_layers, slots=slots, context_capacity=context_capacity,
                                    max_query_tokens=max_query_tokens, heads=cfg.num_key_value_heads,
-                                   dim=cfg.head_dim, dtype=embed.dtype, device=embed.device, chunk=chunk)
+                                   dim=cfg.head_dim, dtype=embed.dtype, device=embed.device, chunk=chunk,
+                                   shared_prefixes=shared_prefixes)
         # The kernel object the reference's session guards read
         # (packed_sampling.py:110-115): the capacity-tail drop-in of
         # _native_attention.  Verification itself runs the fused store launch.
@@ -406,6 +407,14 @@ class PersistentQwenTarget:
         self._ready()
         self.store.remove_request(self._handles[request])
         del self._handles[request]
+
+    def share_prefix(self, source, request, length):
+        """Give the empty `request` the first `length` committed rows of `source`
+        (PersistentTargetKV.share_prefix; no reference counterpart): a prompt that
+        requests share is computed once, and the rest of each one's goes through verify and
+        commit.  With shared_prefixes=True the rows are also attended once per round."""
+        self._ready()
+        self.store.share_prefix(self._handles[source], self._handles[request], length)
 
     def reset(self):
         """Release every request incarnation; bucket addresses stay."""

@@ -118,8 +118,8 @@ class LogitControls:
 
     def __init__(self, device, vocab, *, repetition=1.0, presence=0.0, frequency=0.0, bias=None, masked=None,
                  requests=None):
-        if type(vocab) is not int or not 1 <= vocab < 2 ** 31:
-            raise ValueError('vocab must be a positive integer')
+        if type(vocab) is not int or not 1 <= vocab <= 2 ** 30:
+            raise ValueError('vocab must be an integer in [1, 2^30]')
         per_request = [x for x in (repetition, presence, frequency, bias) if x is not None and not isinstance(x, Real)]
         lengths = {len(x) for x in per_request}
         if requests is not None:

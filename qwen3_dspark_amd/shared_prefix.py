@@ -41,7 +41,7 @@ MAX_PREFIX_SEGMENTS = 32
 # prompts of up to 100 tokens over 2,000 rows 27 and 22 us, 3 of 400 over 3,000 65 and 61, 64 requests
 # over 8,192 56 and 57.
 PREFIX_SEGMENT_COST = 400
-PREFIX_TILES = 1024           # partial tiles that prefix segments may take (more where one segment each needs it)
+PREFIX_TILES = 512            # partial tiles that prefix segments may take (more where one segment each needs it)
 TOKEN_INTS = 4
 
 SharedCapacity = namedtuple('SharedCapacity', 'run_records prompt_records runs requests columns tiles prefix_tiles items '
@@ -108,7 +108,7 @@ def shared_capacity(n_req, query_tokens, max_q, n_cu):
     slots = max(XCDS, RESIDENT_PER_CU * n_cu // 8 // XCDS * XCDS)
     prompts = max_q > DECODE_TOKENS
     width = n_req + (query_tokens // DECODE_TOKENS if prompts else 0)
-    prefix = max(PREFIX_TILES, width)
+    prefix = max(width, min(PREFIX_TILES, MAX_PREFIX_SEGMENTS * width))
     own = width + n_req + slots + (PROMPT_TOKENS // DECODE_TOKENS * slots if prompts else 0)
     tiles = query_tokens // PROMPT_TOKENS + n_req                      # 32-token tiles at most
     return SharedCapacity(n_req + slots - 1, n_req + slots - 1 if prompts else 0, slots, n_req,
@@ -214,16 +214,26 @@ def shared_plan(query_lengths, key_lengths, starts, groups, n_cu, capacity, *, x
     place = {r: i for i, r in enumerate(prompts)}
     columns = _prompt_columns(rows, [(place[r], own_from[r] + a, own_from[r] + b) for r, a, b in loose], c.run_records, True)
 
+    start = 0
     for group, p in zip(groups, parts):
-        start = len(tokens) // TOKEN_INTS
-        for r in group.members:
-            for t in range(query_lengths[r]):
-                tokens += (q0[r] + t, slot[r] + t // DECODE_TOKENS, t % DECODE_TOKENS, width[r])
-        count = len(tokens) // TOKEN_INTS - start
-        cuts = [i * (group.length // PREFIX_TILE) // p * PREFIX_TILE for i in range(p + 1)]
-        for i in range(p):
-            for t in range(0, count, PROMPT_TOKENS):
-                items += (group.slot, cuts[i], cuts[i + 1], i, start + t, min(PROMPT_TOKENS, count - t), 0, 0)
+        m = np.array(group.members)
+        q, w, s = (np.array([x[r] for r in group.members], dtype=np.int32) for x in (query_lengths, width, slot))
+        count = int(q.sum())
+        ends = np.cumsum(q, dtype=np.int32)
+        t = np.arange(count, dtype=np.int32) - np.repeat(ends - q, q)          # the token's place in its request
+        rows = np.array(q0, dtype=np.int32)[m]
+        tokens.append(np.stack((np.repeat(rows, q) + t, np.repeat(s, q) + t // DECODE_TOKENS, t % DECODE_TOKENS,
+                                np.repeat(w, q)), 1))
+        tile = np.arange(0, count, PROMPT_TOKENS, dtype=np.int32)
+        cuts = np.arange(p + 1, dtype=np.int32) * (group.length // PREFIX_TILE) // p * PREFIX_TILE
+        some = np.zeros((p, len(tile), WORK_INTS), dtype=np.int32)           # all token tiles of a segment together
+        some[:, :, 0], some[:, :, 3] = group.slot, np.arange(p)[:, None]
+        some[:, :, 1], some[:, :, 2] = cuts[:-1, None], cuts[1:, None]
+        some[:, :, 4], some[:, :, 5] = start + tile, np.minimum(PROMPT_TOKENS, count - tile)
+        items.append(some.reshape(-1, WORK_INTS))
+        start += count
+    items = np.concatenate(items).reshape(-1) if items else ()
+    tokens = np.concatenate(tokens).reshape(-1) if tokens else ()
 
     if (first > c.run_records or len(loose) > c.prompt_records or len(per_run) > c.runs or n > c.requests
             or len(columns) > 2 * c.columns or used > c.tiles or len(items) > WORK_INTS * c.items

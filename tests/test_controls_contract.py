@@ -21,7 +21,7 @@ def test_rules_are_checked_before_the_device(kw, match):
 
 
 def test_vocabulary_and_device():
-    for vocab in (0, -1, 2 ** 31, 1.5, True):
+    for vocab in (0, -1, 2 ** 30 + 1, 1.5, True):
         with pytest.raises(ValueError, match='vocab'):
             LogitControls('cpu', vocab)
     with pytest.raises(RuntimeError, match='gfx950'):
@@ -41,7 +41,7 @@ def test_entry_point_checks():
         return lib.dspark_logit_controls(*args.values()), lib.dspark_last_error().decode()
     for kw, match in ((dict(logits=None), 'null'), (dict(history=None), 'null'), (dict(n_req=0), 'n_req'),
                       (dict(n_req=65536), 'n_req'), (dict(layout=None), 'null'), (dict(rows=0), 'rows'), (dict(text_tokens=-1), 'rows'),
-                      (dict(host_layout=1, n_req=129), 'host memory'), (dict(vocab=0), 'vocab'), (dict(row_stride=99), 'vocab'),
+                      (dict(host_layout=1, n_req=129), 'host memory'), (dict(vocab=0), 'vocab'), (dict(vocab=2 ** 30 + 1, row_stride=2 ** 31, out_stride=2 ** 31), 'vocab'), (dict(row_stride=99), 'vocab'),
                       (dict(out_stride=99), 'vocab'), (dict(dtype=2), 'dtype'), (dict(dtype=1), 'out_dtype'),
                       (dict(history_bytes=2), 'history'), (dict(history_stride=-1), 'mask row'),
                       (dict(allowed_stride=3), 'mask row'), (dict(out=fake, out_stride=104), 'in place'),

@@ -83,6 +83,17 @@ def test_against_the_formula(lengths, ids, rank):
     assert all(torch.equal(a[bare], b[bare]) for a, b in zip(got, plain))
 
 
+@pytest.mark.parametrize('tokens', [300, 600])
+@pytest.mark.parametrize('rank', [64, 100])
+def test_high_ranks_of_many_tokens(tokens, rank):
+    from qwen3_dspark_amd.adapters import AdapterBatch
+    layer = Layer(4, rank, seed=tokens)
+    lengths = [tokens - 21, 1, 7, 13]
+    x, positions, rope = layer.inputs(tokens)
+    got = layer.prologue(x, positions, rope=rope, adapters=layer.adapters, batch=AdapterBatch(DEV, lengths, [3, 0, -1, 1]))
+    check(got, layer.expected(x, rope, lengths, [3, 0, -1, 1]))
+
+
 @pytest.mark.parametrize('hidden,rank,adapters', [(128, 256, 2), (256, 3, 1), (2048, 64, 5)])
 def test_sizes(hidden, rank, adapters):
     from qwen3_dspark_amd.adapters import AdapterBatch

@@ -207,6 +207,17 @@ def test_small_groups_are_attended_request_by_request(monkeypatch):
     check(store.attend(tx, 0, q, keys=nk, values=nv), want)
 
 
+def test_counters_and_workspace():
+    from qwen3_dspark_amd.persistent_kv import Bucket
+    store, handles, gen = build([(1000, [3, 40, 0]), (0, [70])])
+    bucket = Bucket((7, 2, 1, 40), (2000,) * 4, 'round')
+    store.register_bucket(bucket)
+    assert store.workspace_bytes(bucket) == store.workspace(bucket).nbytes()
+    work = store.work(store.begin(handles, bucket))
+    assert work['logical_active_key_tokens'] == 3 * 1000 + 3 + 40 + 70 + 50
+    assert work['fused_attention_key_rows_per_layer'] == work['logical_active_key_tokens'] - 2 * 960
+
+
 def test_far_slots():
     """Elements past 2^31: 48 slots of 65,536 rows; the group is the last four."""
     from qwen3_dspark_amd.persistent_kv import Bucket
@@ -331,6 +342,51 @@ def test_a_round_of_tenants():
         before = [store.length(h) for h in handles]
         store.commit(tx, {h: len(x.tokens) for h, x in zip(handles, done)})
         assert [store.length(h) - b for h, b in zip(handles, before)] == [len(x.tokens) for x in done]
+
+
+def test_the_persistent_target():
+    """Requests of a PersistentQwenTarget that share a prompt: hidden states and logits of the rest of
+    each prompt and of later rounds are those of requests that computed all of theirs."""
+    from qwen3_dspark_amd.persistent_kv import Bucket
+    from test_gpu_hf_hooks import close, tiny_qwen3
+    from test_gpu_persistent_target import ids, make_target
+    rng = np.random.default_rng(7)
+    prompt, rests = rng.integers(0, 512, 130).tolist(), [rng.integers(0, 512, n).tolist() for n in (3, 20, 9)]
+    rounds = [[rng.integers(0, 512, 7).tolist() for _ in range(3)] for _ in range(2)]
+    names, logits = ['a', 'b', 'c'], []
+    for shared in (False, True):
+        target = make_target(tiny_qwen3()[1], slots=4, context_capacity=512, max_query_tokens=512, graph_backend=None,
+                             max_graph_buckets=0, graph_byte_budget=0, shared_prefixes=shared)
+        for n in names:
+            target.add_request(n)
+        lengths = tuple(len(r) + (0 if shared else 130) for r in rests)
+        first = Bucket(lengths, (130,) * 3, 'rest')
+        step = Bucket((7,) * 3, (230,) * 3, 'round')
+        for b in (first, step):
+            target.register_bucket(b)
+        if shared:
+            target.add_request('prompt')
+            alone = Bucket((130,), (0,), 'prompt')
+            target.register_bucket(alone)
+            target.release_features(target.prefill({'prompt': ids(prompt)}, bucket=alone))
+            for n in names:
+                target.share_prefix('prompt', n, 130)
+            target.remove_request('prompt')
+            assert target.lengths == dict.fromkeys(names, 130)
+        got = []
+        f = target.verify({n: ids(r if shared else prompt + r) for n, r in zip(names, rests)}, bucket=first)
+        got += [target.predict(f)[n][0, -len(r):].float() for n, r in zip(names, rests)]
+        target.commit(f, {n: x for n, x in zip(names, lengths)})
+        target.release_features(f)
+        for new in rounds:
+            f = target.verify({n: ids(x) for n, x in zip(names, new)}, bucket=step)
+            got += [x[0].float() for x in target.predict(f).values()]
+            target.commit(f, dict(zip(names, (7, 2, 5))))
+            target.release_features(f)
+        logits.append(got)
+        target.close()
+    for x, y in zip(*logits):
+        close(y.cpu(), x.cpu(), 'logits')        # the gate of one such model against a float32 one
 
 
 def test_refusals():
