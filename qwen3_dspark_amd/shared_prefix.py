@@ -7,14 +7,14 @@ copied from another request (PersistentTargetKV.share_prefix).  A lineage lists,
 no end.  Committed rows never change, so two requests hold the same rows up to the
 position where their lineages part.
 
-Groups.  Requests with a common first origin are candidates for one group, which
-shares the rows that all of its members hold; members that would shorten it more than
-they gain stay out (shared_groups).
+Groups.  A request is in one group at most, whose members share the rows that all of them
+hold: of a system prompt for many and a document for some of these, each request
+shares one or the other, by what saves more rows (shared_groups).
 
 Plan.  Runs and prompt columns over each request's own keys, as in a mixed plan
 (schedule.mixed_plan), whose records start at the prefix's end, with partial slots for the
 prefix's segments ahead of the request's own; and a list of prefix items
-(dspark_prefix_attn_partials in include/dspark_amd.h).  A request of a group always
+(dspark_shared_attn_fwd in include/dspark_amd.h).  A request of a group always
 has partials, at least one of the prefix and one of its own keys.
 """
 from collections import namedtuple
@@ -43,6 +43,7 @@ MAX_PREFIX_SEGMENTS = 32
 PREFIX_SEGMENT_COST = 400
 PREFIX_TILES = 512            # partial tiles that prefix segments may take (more where one segment each needs it)
 TOKEN_INTS = 4
+MAX_BRANCHES = 16             # forks below forks that are looked at for groups of their own
 
 SharedCapacity = namedtuple('SharedCapacity', 'run_records prompt_records runs requests columns tiles prefix_tiles items '
                                               'tokens')
@@ -82,18 +83,53 @@ def shared_groups(lineages, contexts, slots):
         families.setdefault(lineage[0][0], []).append(r)
     groups = []
     for members in families.values():
-        # Everyone's lineage starts with the family's origin; rows in common with it all are
-        # the least of where the first spans end.
-        span = {r: min(contexts[r], contexts[r] if lineages[r][0][1] is None else lineages[r][0][1]) for r in members}
-        while len(members) > 1:
-            members.sort(key=lambda r: (-span[r], r))
-            best = max(range(2, len(members) + 1), key=lambda n: (n - 1) * (span[members[n - 1]] // PREFIX_TILE))
-            chosen = members[:best]
-            rows = span[chosen[-1]] // PREFIX_TILE * PREFIX_TILE
-            if rows == 0 or (best - 1) * rows < MIN_SAVED:
-                break
-            groups.append(Group(sorted(chosen), rows, slots[min(chosen)]))
-            members = members[best:]
+        if len(members) > 1:
+            groups += _groups_from(lineages, contexts, members, 0, 0)
+    return [Group(sorted(members), rows, slots[min(members)]) for members, rows in groups]
+
+
+def _saved(groups):
+    return sum((len(members) - 1) * rows for members, rows in groups)
+
+
+def _groups_from(lineages, contexts, members, depth, branches):
+    """Groups among requests whose lineages are the same up to span `depth`, whose origin they
+    have in common too: all of them there, or those of a branch whose lineages stay the
+    same for longer apart from the rest, whichever saves more rows."""
+    while True:
+        deeper = {}
+        for r in members:
+            if depth + 1 < len(lineages[r]):
+                deeper.setdefault((lineages[r][depth][1], lineages[r][depth + 1][0]), []).append(r)
+        if len(deeper) != 1 or len(*deeper.values()) < len(members):
+            break
+        depth += 1                                             # nobody leaves here
+    reach = {r: contexts[r] if lineages[r][depth][1] is None else min(contexts[r], lineages[r][depth][1]) for r in members}
+    chosen, here = [], _groups_at(members, reach)
+    for branch in deeper.values():
+        if len(branch) < 2 or branches == MAX_BRANCHES:
+            continue
+        apart = _groups_from(lineages, contexts, branch, depth + 1, branches + 1)
+        inside = {r for group, _ in apart for r in group}
+        rest = [r for r in members if r not in inside]
+        without = _groups_at(rest, reach)
+        if apart and _saved(apart) + _saved(without) > _saved(here):
+            members, here = rest, without
+            chosen += apart
+    return chosen + here
+
+
+def _groups_at(members, reach):
+    """[(members, rows)] of requests that have all rows in common up to where each one's reach
+    ends: those who would shorten a group more than they gain stay out of it."""
+    groups, members = [], sorted(members, key=lambda r: (-reach[r], r))
+    while len(members) > 1:
+        best = max(range(2, len(members) + 1), key=lambda n: (n - 1) * (reach[members[n - 1]] // PREFIX_TILE))
+        rows = reach[members[best - 1]] // PREFIX_TILE * PREFIX_TILE
+        if rows == 0 or (best - 1) * rows < MIN_SAVED:
+            break
+        groups.append((members[:best], rows))
+        members = members[best:]
     return groups
 
 

@@ -162,6 +162,35 @@ def test_members_that_would_shorten_a_group_stay_out():
     assert shared_groups([a], [5000], [0]) == []
 
 
+def test_forks_below_forks():
+    """64 rows of a system prompt, on which one request puts a document that two others take
+    over; then the same with more requests on the system prompt alone."""
+    system, doc = ((0, None),), inherited(((0, None),), 64, 1)
+    lineages = [doc, inherited(doc, 8000, 2), inherited(doc, 8100, 3)]
+    groups = shared_groups(lineages, [8500, 8000, 8100], [7, 8, 9])
+    assert [tuple(g) for g in groups] == [([0, 1, 2], 8000, 7)]
+    lineages += [inherited(system, 64, 4), inherited(system, 60, 5), system]
+    groups = shared_groups(lineages, [8500, 8000, 8100, 70, 60, 70], [7, 8, 9, 1, 2, 3])
+    assert sorted(map(tuple, groups)) == [([0, 1, 2], 8000, 7), ([3, 5], 64, 1)]
+    # 40 share 1,024 rows of the system prompt, 3 of which 1,088 in all: those stay
+    doc = inherited(system, 1024, 1)
+    lineages = [doc, inherited(doc, 1088, 2), inherited(doc, 1088, 3), *(inherited(system, 1024, 10 + r) for r in range(37))]
+    groups = shared_groups(lineages, [1100] * 40, list(range(40)))
+    assert [(len(g.members), g.length) for g in groups] == [(40, 1024)]
+
+
+def test_long_chains_of_forks():
+    chain = [((0, None),)]
+    for r in range(1, 1500):
+        chain.append(inherited(chain[-1], 64 * r, r))          # each has 64 rows of its own
+    n = len(chain)
+    groups = shared_groups(chain, [64 * (r + 1) for r in range(n)], list(range(n)))
+    held = [r for g in groups for r in g.members]
+    assert len(held) == len(set(held)) and all(g.length <= 64 * (min(g.members) + 1) for g in groups)
+    groups = shared_groups([chain[-1], chain[-1][:-1] + ((9999, None),)], [64 * n] * 2, [0, 1])
+    assert [tuple(g) for g in groups] == [([0, 1], 64 * (n - 1), 0)]
+
+
 def test_groups_that_would_save_little_are_none(monkeypatch):
     monkeypatch.undo()
     a = ((0, None),)
