@@ -472,7 +472,8 @@ int dspark_sample_rows(const double* probs, int rows, int vocab, const double* u
  *   y -= c alpha_f + [c > 0] alpha_p, c: occurrences behind the prompt;
  *   y += bias of v; and y = fill where the row's mask does not allow v.
  * history: int32 or int64 (history_bytes) rows, history_stride
- * elements apart; tokens outside the vocabulary are passed over.  penalties:
+ * elements apart; at most 2^28 tokens a text, those outside the
+ * vocabulary passed over.  penalties:
  * double [3][n_req]: rho, alpha_p, alpha_f.  Biases of request r: entries bias_start[r] ..
  * bias_start[r+1] of bias_token / bias_value, at most 65,535, no token twice.  allowed (optional):
  * allowed_stride words a row, token v is bit v % 32 of word v / 32.  A row whose mask

@@ -175,6 +175,27 @@ class HostStaging:
         return out
 
 
+class Prepared:
+    """Device tensors that are written once, on the stream that is current here, and read by
+    later calls on any stream (`on` each).  A captured launch is left to its capture, which
+    starts behind a synchronization, and to the graph's owner, who keeps them."""
+
+    def __init__(self, device, *tensors):
+        self.tensors = tensors
+        stream = torch.cuda.current_stream(device)
+        self.stream, self.event = stream.cuda_stream, torch.cuda.Event()
+        self.event.record(stream)
+
+    def on(self, device, handle):
+        """Before a launch on the stream of this handle, the device's current one."""
+        if handle == self.stream or torch.cuda.is_current_stream_capturing():
+            return
+        stream = torch.cuda.current_stream(device)
+        stream.wait_event(self.event)
+        for t in self.tensors:
+            t.record_stream(stream)
+
+
 _STAGING = {}
 _STAGING_LOCK = threading.Lock()
 

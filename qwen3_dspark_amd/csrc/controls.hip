@@ -171,7 +171,7 @@ __global__ __launch_bounds__(T) void logit_controls_kernel(ControlArgs a) {
   // for which all arguments would be copied to scratch memory.
   const uint32_t fill_bits = (uint32_t)__builtin_amdgcn_readfirstlane((int)__builtin_bit_cast(uint32_t, a.fill));
   const float fill = __builtin_bit_cast(float, fill_bits);
-  const uint32_t fill_word = OUT == 1 ? fill_bits : (fill_bits >> 16) * 0x10001u;
+  const uint32_t fill_word = OUT == 1 ? fill_bits : __builtin_bit_cast(uint16_t, (bf16)fill) * 0x10001u;
   for (int i0 = tid; i0 < rows * GROUPS; i0 += T * LC_FLIGHT) {
     u32x4 raw[LC_FLIGHT];
     uint32_t keep[LC_FLIGHT];

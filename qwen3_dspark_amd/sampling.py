@@ -39,7 +39,7 @@ from operator import add, gt
 import torch
 
 from . import _native
-from ._device import Workspace, require_gfx950, upload
+from ._device import Prepared, Workspace, require_gfx950, upload
 
 PROBABILITY_POLICY = 'float64_softmax_normalize_cdf_v1'
 _EXTRA = {0: None, 1: 'residual', 2: 'bonus'}
@@ -54,6 +54,7 @@ _ERRORS = {
 }
 MAX_PROPOSAL = 255
 _LOWEST = {t: torch.finfo(t).min for t in (torch.bfloat16, torch.float32)}
+_MAX_TEXT = 2 ** 28          # occurrences are counted in 29 bits
 _LAYOUT_ON_HOST = 128        # requests whose layout goes with the launch of the controls
 
 
@@ -150,17 +151,16 @@ class LogitControls:
                 tokens.append(token)
                 values.append(float(value))
             start.append(len(tokens))
-        if masked is not None and (isinstance(masked, bool) or not isinstance(masked, Real) or masked != masked):
-            raise ValueError('masked must be a number or None')
+        if masked is not None and (isinstance(masked, bool) or not isinstance(masked, Real) or masked != masked
+                                   or torch.finfo(torch.float32).max < abs(masked) < math.inf):
+            raise ValueError('masked must be a number of the fp32 range, an infinity or None')
         self.masked = masked
         self.device = require_gfx950(device)
         self._penalties = upload(self.device, rules, torch.float64)
         self._bias_start = upload(self.device, start)
         self._bias_token = upload(self.device, tokens)
         self._bias_value = upload(self.device, values, torch.float64)
-        self._stream = _native.stream_handle(self.device)
-        self._uploaded = torch.cuda.Event()
-        self._uploaded.record(torch.cuda.current_stream(self.device))
+        self._ready = Prepared(self.device, self._penalties, self._bias_start, self._bias_token, self._bias_value)
         self._none, self._each = array('i', [0] * n), array('i', range(n))
 
     def __call__(self, logits, history, *, lengths, prompt_lengths=None, counts=None, tokens=None, slots=None,
@@ -179,10 +179,13 @@ class LogitControls:
         if torch.cuda.is_current_stream_capturing():
             raise ValueError('The lengths are uploaded with each call, which a captured graph cannot repeat')
         n = self.requests
-        lengths = array('i', lengths)
-        prompts = self._none if prompt_lengths is None else array('i', prompt_lengths)
-        counts = self._none if counts is None else array('i', counts)
-        slots = self._each if slots is None else array('i', slots)
+        try:
+            lengths = array('i', lengths)
+            prompts = self._none if prompt_lengths is None else array('i', prompt_lengths)
+            counts = self._none if counts is None else array('i', counts)
+            slots = self._each if slots is None else array('i', slots)
+        except (TypeError, OverflowError):
+            raise ValueError('Lengths, prompt lengths, proposal lengths and texts must be sequences of integers') from None
         if len(lengths) != n:
             raise ValueError(f'These controls rule {n} requests')
         if not len(prompts) == len(counts) == len(slots) == n:
@@ -199,6 +202,8 @@ class LogitControls:
         if (min(slots) < 0 or max(slots) >= texts or min(prompts) < 0 or max(lengths) > capacity
                 or any(map(gt, prompts, lengths))):
             raise ValueError('Texts must lie within history, prompts within their texts')
+        if max(lengths) > _MAX_TEXT:
+            raise ValueError('At most 2^28 tokens per text')
         if total and (not isinstance(tokens, torch.Tensor) or tokens.dtype != torch.long or tokens.shape != (total,)
                       or tokens.device != self.device):
             raise ValueError('tokens must be the proposed tokens, int64, on the controls\' device')
@@ -219,8 +224,7 @@ class LogitControls:
         if logits.stride(0) < self.vocab:
             raise ValueError('Logit rows must not overlap')
         stream = _native.stream_handle(self.device)
-        if stream != self._stream:
-            torch.cuda.current_stream(self.device).wait_event(self._uploaded)
+        self._ready.on(self.device, stream)
         layout = array('i', accumulate(map(add, counts, repeat(1)), initial=0)) + slots + lengths + prompts
         here = n <= _LAYOUT_ON_HOST
         place = layout.buffer_info()[0] if here else (layout := upload(self.device, layout)).data_ptr()

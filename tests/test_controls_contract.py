@@ -14,7 +14,7 @@ from qwen3_dspark_amd.sampling import LogitControls
     (dict(repetition=[1.0, 1.1], presence=[0.0]), 'same number'), (dict(repetition=[]), 'same number'),
     (dict(repetition=[1.0], requests=2), 'same number'), (dict(requests=0), 'same number'),
     (dict(bias=[{100: 1.0}]), 'vocabulary'), (dict(bias=[{-1: 1.0}]), 'vocabulary'), (dict(bias=[{1.5: 1.0}]), 'vocabulary'),
-    (dict(bias=[{1: float('-inf')}]), 'finite'), (dict(bias=[{i: 1.0 for i in range(65536)}]), '65,535'), (dict(masked=float('nan')), 'masked'), (dict(masked='low'), 'masked')])
+    (dict(bias=[{1: float('-inf')}]), 'finite'), (dict(bias=[{i: 1.0 for i in range(65536)}]), '65,535'), (dict(masked=float('nan')), 'masked'), (dict(masked='low'), 'masked'), (dict(masked=1e39), 'masked'), (dict(masked=-10 ** 400), 'masked')])
 def test_rules_are_checked_before_the_device(kw, match):
     with pytest.raises(ValueError, match=match):
         LogitControls('cpu', 100, **kw)

@@ -182,6 +182,31 @@ def test_two_streams_and_two_calls_at_once():
     check(second, d.expected(), torch.bfloat16)
 
 
+def test_rules_prepared_on_a_busy_stream():
+    b = Batch(20011, [4] * 9, 500, torch.bfloat16, seed=6)
+    work = torch.randn(4096, 4096, device=DEV)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        for _ in range(8):
+            work = work @ work * 1e-2
+        controls = b.controls()
+    got = b.call(controls)
+    del controls
+    torch.cuda.synchronize()
+    check(got, b.expected(), torch.bfloat16)
+
+
+@pytest.mark.parametrize('masked', [-1.0039e4, 2.99e-3, 3.4e38])
+@pytest.mark.parametrize('dtype,out', [(torch.bfloat16, None), (torch.bfloat16, torch.float32), (torch.float32, None)])
+def test_fills_are_rounded_to_the_output(masked, dtype, out):
+    """To nearest, like every value, and alike in whole groups and in the odd ends of rows."""
+    b = Batch(5003, [2, 0], 50, dtype, seed=8, pad=5, masked=masked, out=out)
+    got = b.call(out=None if out is None else torch.empty(b.logits.shape, dtype=out, device=DEV))
+    fill = torch.tensor(masked, dtype=torch.float32).to(b.out_dtype).to(DEV)
+    assert (got[torch.from_numpy(~b.allowed).to(DEV)] == fill).all()
+
+
 def test_the_law_behind_controls():
     """Masked tokens have no probability, a row that allows nothing is refused, and a
     verification of ruled logits is the oracle's."""
@@ -209,13 +234,15 @@ def test_the_law_behind_controls():
         logits_to_probabilities(b.call(), 0.9)
 
 
-def test_refusals():
+def test_refusals(monkeypatch):
+    from qwen3_dspark_amd import sampling
     from qwen3_dspark_amd.sampling import LogitControls
     b = Batch(700, [1, 2], 40, torch.bfloat16, mask=False)
     c = b.controls()
     good = dict(lengths=b.lengths, prompt_lengths=b.prompts, counts=b.counts, tokens=b.proposed)
     for change, match in (
-            (dict(lengths=[1]), 'rule 2 requests'), (dict(lengths=[41, 44]), 'within history'),
+            (dict(lengths=[1]), 'rule 2 requests'), (dict(lengths=[1.0, 2]), 'integers'),
+            (dict(counts=[1, 2 ** 40]), 'integers'), (dict(slots=5), 'integers'), (dict(lengths=[41, 44]), 'within history'),
             (dict(prompt_lengths=[41, 0]), 'within history'), (dict(prompt_lengths=[0]), 'per request'),
             (dict(counts=[1, 1]), 'a row for each'), (dict(counts=[-1, 4]), 'a row for each'),
             (dict(slots=[0, 2]), 'within history'), (dict(tokens=b.proposed.int()), 'int64'),
@@ -239,6 +266,10 @@ def test_refusals():
     with pytest.raises(ValueError, match='255'):
         many(torch.zeros(257, 700, device=DEV), b.history, lengths=[1], counts=[256],
              tokens=torch.zeros(256, dtype=torch.long, device=DEV))
+    monkeypatch.setattr(sampling, '_MAX_TEXT', 39)
+    with pytest.raises(ValueError, match='per text'):
+        b.call(c)
+    monkeypatch.undo()
     graph = torch.cuda.CUDAGraph()
     with pytest.raises(ValueError, match='captured graph'):
         with torch.cuda.graph(graph):
