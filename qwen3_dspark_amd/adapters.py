@@ -17,7 +17,7 @@ from numbers import Real
 
 import torch
 
-from ._device import require_gfx950, upload
+from ._device import Prepared, require_gfx950, upload
 from .kernels import HEAD_DIM, KV_HEADS, Q_HEADS
 
 TILE_TOKENS = 16             # tokens of one adapter per shrinking workgroup
@@ -51,6 +51,7 @@ class AdapterBatch:
         self.device = require_gfx950(device)
         self.token_adapter = upload(self.device, [a for n, a in zip(lengths, ids) for _ in range(n)])
         self.tiles = upload(self.device, [x for t in tiles for x in t])
+        self._ready = Prepared(self.device, self.token_adapter, self.tiles)
 
 
 class QKVAdapters:
@@ -84,6 +85,7 @@ class QKVAdapters:
         for at, t in ((0, b_q), (q, b_k), (q + kv, b_v)):
             self.b[:, at:at + t.shape[1], :rank] = t.detach()
         self.scaling = upload(self.device, [float(x) for x in scaling], torch.float32)
+        self._ready = Prepared(self.device, self.a, self.b, self.scaling)
         self.pointers = (self.a.data_ptr(), self.b.data_ptr(), self.scaling.data_ptr(), n, self.padded_rank, rank)
 
     def check(self, batch, tokens, hidden, device):
@@ -94,6 +96,11 @@ class QKVAdapters:
             raise ValueError('Adapters must have the prologue\'s hidden size and device')
         if batch.largest >= self.count:
             raise ValueError(f'The batch names adapter {batch.largest} of {self.count}')
+
+    def ready(self, batch, stream):
+        """Before the launches on the stream of this handle."""
+        self._ready.on(self.device, stream)
+        batch._ready.on(self.device, stream)
 
     def scratch(self, tokens):
         """Elements of the scaled A x of a batch, two bf16 numbers each."""

@@ -2717,6 +2717,7 @@ extern "C" int dspark_shared_attn_fwd(const void* q, int64_t q_rows, const void*
                  "Q/K/V/out, the prefix list and the workspace must be 16-byte aligned");
   DSPARK_REQUIRE(slot_stride >= 0 && tok_stride >= HD && tok_stride % 8 == 0 && head_stride >= HD && head_stride % 8 == 0,
                  "resident strides must be multiples of 8 elements (token/head strides >= 128)");
+  DSPARK_REQUIRE(tok_stride <= (1 << 28), "the token stride must be at most 2^28 elements");
   DSPARK_REQUIRE(q_rows >= 1 && q_rows <= 0x7fffffffLL, "q_rows must be in [1, 2^31)");
   DSPARK_REQUIRE(max_q >= 1, "max_q must be >= 1");
   DSPARK_REQUIRE(n_work >= 1 && n_groups >= 8 && n_groups <= (1 << 24) && n_groups % 8 == 0 && n_columns >= 0 &&

@@ -16,6 +16,7 @@ import torch
 
 from . import _native
 from ._device import require_gfx950
+from .adapters import QKVAdapters
 from .kernels import HEAD_DIM, KV_HEADS, Q_HEADS
 
 
@@ -97,6 +98,8 @@ class QKVPrologue:
         if (adapters is None) != (batch is None):
             raise ValueError('adapters and batch go together')
         if adapters is not None:
+            if not isinstance(adapters, QKVAdapters):
+                raise ValueError('adapters must be a QKVAdapters')
             adapters.check(batch, t, self.hidden, self.device)
         q = torch.empty((t, Q_HEADS, HEAD_DIM), dtype=torch.bfloat16, device=self.device)
         outs = []
@@ -115,6 +118,7 @@ class QKVPrologue:
         into = (q.data_ptr(), outs[0].data_ptr(), outs[1].data_ptr(), KV_HEADS * HEAD_DIM,
                 _native.stream_handle(self.device))
         if adapters is not None and batch.n_tiles:
+            adapters.ready(batch, into[-1])
             scratch = torch.empty(adapters.scratch(t), dtype=torch.bfloat16, device=self.device)
             _native.call('dspark_qkv_prologue_adapted', *given, *adapters.pointers, batch.token_adapter.data_ptr(),
                          batch.tiles.data_ptr(), batch.n_tiles, scratch.data_ptr(), *into)

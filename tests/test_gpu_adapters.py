@@ -170,6 +170,35 @@ def test_two_streams():
         check(got, b[0].expected(b[1], b[3], lengths, b[4]))
 
 
+def test_prepared_on_a_busy_stream():
+    """Layer and batch made on a stream with work ahead of them, used on another at once, and
+    dropped there while the launches still wait."""
+    from qwen3_dspark_amd.adapters import AdapterBatch
+    reference = Layer(3, 16)
+    x, positions, rope = reference.inputs(84)
+    lengths, ids = [7] * 12, [i % 4 - 1 for i in range(12)]
+    work = torch.randn(4096, 4096, device=DEV)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        for _ in range(8):
+            work = work @ work * 1e-2
+        layer = Layer(3, 16)
+        batch = AdapterBatch(DEV, lengths, ids)
+        weights = torch.cuda.Event()
+        weights.record()
+    torch.cuda.current_stream().wait_event(weights)          # the shared weights are the caller's
+    got = [layer.prologue(x, positions, rope=rope, adapters=layer.adapters, batch=batch) for _ in range(3)]
+    del layer.adapters, batch
+    with torch.cuda.stream(side):                            # what those had, were it free already
+        junk = [torch.full((3, 3, 16, H), 7.0, dtype=torch.bfloat16, device=DEV) for _ in range(4)]
+    torch.cuda.synchronize()
+    assert len(junk) == 4
+    want = reference.expected(x, rope, lengths, ids)
+    for g in got:
+        check(g, want)
+
+
 def test_staged_in_a_transaction():
     from qwen3_dspark_amd.adapters import AdapterBatch
     from qwen3_dspark_amd.persistent_kv import Bucket, PersistentTargetKV
@@ -200,6 +229,8 @@ def test_refusals():
     for other, match in ((AdapterBatch(DEV, [5, 6], [0, 1]), '12 tokens'), (AdapterBatch(DEV, [5, 7], [0, 2]), 'adapter 2 of 2')):
         with pytest.raises(ValueError, match=match):
             layer.prologue(x, positions, adapters=layer.adapters, batch=other)
+    with pytest.raises(ValueError, match='QKVAdapters'):
+        layer.prologue(x, positions, adapters=[layer.adapters], batch=batch)
     with pytest.raises(ValueError, match='hidden size'):
         layer.prologue(x, positions, adapters=Layer(2, 16, 256).adapters, batch=batch)
     given = [t for p in 'qkv' for t in (layer.a[p], layer.b[p])]

@@ -1,13 +1,14 @@
 """Lineages, groups and plans of requests that share committed rows (CPU): every plan
 covers each request's keys exactly once, its partial tiles are disjoint and within the
 capacity, and its regions hold what the kernels read."""
+import ctypes
 import random
 
 import pytest
 import torch
 
 from kv_fake import store
-from qwen3_dspark_amd import shared_prefix
+from qwen3_dspark_amd import _native, shared_prefix
 from qwen3_dspark_amd.schedule import REQ_INTS, WORK_INTS
 from qwen3_dspark_amd.shared_prefix import (PREFIX_TILE, common_rows, inherited, mixed_part_ints, shared_capacity,
                                             shared_groups, shared_ints, shared_plan)
@@ -238,3 +239,32 @@ def test_constructor_refusals():
         PersistentTargetKV(**dims, shared_prefixes=1)
     with pytest.raises(RuntimeError, match='gfx950'):
         PersistentTargetKV(**dims, shared_prefixes=True, device='cpu')
+
+
+def test_entry_point_checks():
+    lib = _native.load()
+    fake = ctypes.c_void_p(1 << 20)                # never dereferenced
+
+    def call(**kw):
+        args = dict(q=fake, q_rows=8, k_res=fake, v_res=fake, k_new=fake, v_new=fake, k_scr=fake, v_scr=fake, n_req=1,
+                    slot_stride=8 * 128 * 64, tok_stride=128, head_stride=128 * 64, max_q=8, scale=0.1, work=fake, n_work=1,
+                    n_groups=8, n_columns=0, prefixes=fake, max_items=1, max_tokens=8, members=8, turn=8, part_tiles=1,
+                    out=fake, workspace=fake, workspace_bytes=1 << 20, stream=None)
+        args.update(kw)
+        return lib.dspark_shared_attn_fwd(*args.values()), lib.dspark_last_error().decode()
+    odd = ctypes.c_void_p((1 << 20) + 8)
+    for kw, match in (*((dict.fromkeys((x,)), 'null') for x in ('q', 'k_res', 'v_res', 'k_new', 'v_new', 'work', 'prefixes',
+                                                                'out', 'workspace')),
+                      (dict(k_scr=None), 'together'), (dict(v_scr=None), 'together'),
+                      *((dict.fromkeys((x,), odd), 'aligned') for x in ('q', 'v_res', 'k_new', 'v_scr', 'prefixes', 'out',
+                                                                        'workspace')),
+                      (dict(slot_stride=-8), 'strides'), (dict(tok_stride=64), 'strides'), (dict(tok_stride=132), 'strides'),
+                      (dict(head_stride=4), 'strides'), (dict(tok_stride=(1 << 28) + 8), 'token stride'),
+                      (dict(q_rows=0), 'q_rows'), (dict(q_rows=2 ** 31), 'q_rows'), (dict(max_q=0), 'max_q'),
+                      (dict(n_work=0), 'n_work'), (dict(n_groups=12), 'n_groups'), (dict(n_groups=0), 'n_groups'),
+                      (dict(n_columns=-1), 'n_columns'), (dict(max_items=0), 'max_items'), (dict(max_tokens=0), 'max_tokens'),
+                      (dict(members=0), 'members'), (dict(turn=0), 'turn'), (dict(turn=65537), 'turn'),
+                      (dict(n_req=0), 'n_req'), (dict(scale=float('nan')), 'scale'), (dict(part_tiles=0), 'part_tiles'),
+                      (dict(workspace_bytes=100), 'workspace too small')):
+        rc, message = call(**kw)
+        assert rc == -1 and match in message, (kw, message)
