@@ -2100,9 +2100,21 @@ __global__ __launch_bounds__(PF_WAVES * WAVE, 2) void prefill_attn_kernel(Varlen
 // mask, and cuts at multiples of 64 keys leave no partial stage.
 //
 // Work: a workgroup takes items (32 query tokens of a group, one key segment) of KV
-// head blockIdx.x % 8, which its XCD's L2 then holds for all of the group's token
-// tiles; the grid is fixed and the list says how many there are, so that a captured
-// launch serves every transaction.  Tiles and stages as in prefill_attn_kernel.
+// head blockIdx.x % 8, whose keys its XCD's L2 then holds for all of the group's token
+// tiles; the grid is fixed and the list says how many items there are, so that a captured
+// launch serves every transaction.  Tiles and stages as in prefill_attn_kernel.  The items
+// go in the launch of the requests' own keys: in a launch of their own, 16 requests x 7 tokens
+// over 2,048 shared rows 25.5 us a call, together 20.4, 64 over 8,192 75 / 55.
+//
+// Bound by the vector unit, then the matrix unit: 12 prompts of 2,645 tokens over two
+// prefixes of 5,379 and 6,000 rows (126 GFLOP) take 166 to 192 us, 0.65 to 0.75 PFLOP/s, in which vector instructions issue
+// in 48 % of the cycles (half of those the exponentials') and MFMAs run in 38 %; the same work
+// request by request 234 us.  64 requests of 1 to 8 tokens over 8,192 rows: 55 us with their own
+// keys (190 MB, 37 us), 354 request by request.
+//
+// Tried: 64 tokens per item on 8 waves with one barrier per two stages, 200 us for the
+// prompts; on 4 waves that each take both halves of a stage (half the LDS fills and barriers),
+// 174 with 48 B of spills.  So neither the fills (15 TB/s from L2) nor the barriers bound it.
 struct PrefixArgs {
   const bf16* q;           // [nq, 16, 128]
   const bf16* k;           // resident layer
@@ -2116,8 +2128,11 @@ struct PrefixArgs {
 };
 
 // Probabilities of a tile of raw scores x against m_use, rounded to bf16 for PV; the
-// denominator sums them unrounded.  One operand, as in the 8-token workgroups that attend
-// the requests' own keys: ONEOP.
+// denominator sums them unrounded.  One bf16 operand, as in the 8-token workgroups: an output is
+// off by at most 2^-8 of the mean |v| under its probabilities, as much as by its own rounding.
+// Errors against 64 bits over the cases above 2.2e-3 to 2.3e-3 with one operand, 1.7e-3 with two
+// (the value and its rest, as prompts take it), which cost 34 -> 42 us over the 64 requests'
+// prefix and 155 -> 201 us over the prompts'.
 __device__ __forceinline__ void prefix_probs(PairState& st, const f32x16& x, float m_use, float scale_log2, bf16x8 (&p)[2]) {
   float ps[2] = {0.f, 0.f};
   #pragma unroll
@@ -2135,7 +2150,8 @@ __device__ __forceinline__ void prefix_probs(PairState& st, const f32x16& x, flo
 }
 
 // prefill_full_tile with one operand: the scores of the next tile beside this one's maximum
-// and exponentials, then PV.
+// and exponentials, then PV.  Its order of instructions is worth little here: without the groups
+// below, with the V reads behind the scores or 0, 3 or 5 steps of them ahead +-3 %.
 __device__ __forceinline__ f32x16 prefix_tile(PairState& st, const bf16x8 (&qf)[8], const f32x16& x, uint32_t ka,
                                               uint32_t va, float scale_log2) {
   bf16x8 kf[8], vt[2][4];
