@@ -310,8 +310,8 @@ int dspark_qkv_prologue(const void* x, const void* wq, const void* wk, const voi
  * beside the shared projections; no reference counterpart.  Token t of adapter a =
  * token_adapter[t] (-1: none) projects with W + s_a B_a A_a in place of W, in all of q, k and
  * v, before the norm and RoPE.  Two launches: one forms u = s_a A_a x_t for the tokens of
- * the tiles, int32 [n_tiles][4] records (first token, tokens (1 to 16), adapter, 0) that
- * cover every token of an adapter once, the other adds B_a u to the shared
+ * the tiles, int32 [n_tiles][4] records (first token, tokens (1 to tile_tokens, which is 16
+ * or 32), adapter, 0) that cover every token of an adapter once, the other adds B_a u to the shared
  * projection's accumulators.
  * adapter_a: [adapters][3 (q, k, v)][rank][hidden], adapter_b: [adapters][4096 (q, k, v
  * outputs)][rank] bf16, scaling float [adapters]; rank 16, 32 or a multiple of 64 up to 256;
@@ -323,7 +323,8 @@ int dspark_qkv_prologue_adapted(const void* x, const void* wq, const void* wk, c
                                 const void* k_norm, const float* inv_freq, const int64_t* positions,
                                 const float* rope, int tokens, int hidden, float eps, const void* adapter_a,
                                 const void* adapter_b, const float* scaling, int adapters, int rank, int own_rank,
-                                const int32_t* token_adapter, const int32_t* tiles, int n_tiles, void* u, void* q_out,
+                                const int32_t* token_adapter, const int32_t* tiles, int n_tiles, int tile_tokens,
+                                void* u, void* q_out,
                                 void* k_out, void* v_out, int64_t kv_row_stride, void* stream);
 
 /*

@@ -53,7 +53,7 @@ SIGNATURES = {
     'dspark_rows_pack': (_I, [_P, _P, _I, _I, _L, _L, _P, _P, _P]),
     'dspark_qkv_prologue': (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _F, _P, _P, _P, _L, _P]),
     'dspark_qkv_prologue_adapted': (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _F, _P, _P, _P, _I, _I, _I, _P, _P, _I,
-                                         _P, _P, _P, _P, _L, _P]),
+                                         _I, _P, _P, _P, _P, _L, _P]),
     'dspark_rope_table': (_I, [_P, _P, _I, _P, _P]),
     'dspark_draft_kv_project': (_I, [_P, _I, _I, _P, _P, _I, _P, _P, _I, _F, _F, _P, _P, _L, _L, _L, _P, _P]),
     'dspark_draft_rows_bytes': (_L, [_I]),

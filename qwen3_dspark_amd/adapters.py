@@ -20,7 +20,8 @@ import torch
 from ._device import Prepared, require_gfx950, upload
 from .kernels import HEAD_DIM, KV_HEADS, Q_HEADS
 
-TILE_TOKENS = 16             # tokens of one adapter per shrinking workgroup
+TILE_TOKENS = (16, 32)       # tokens of one adapter per shrinking workgroup, of small and of large calls
+SMALL_PAIRS = 256            # (tile, 16 ranks) pairs of small calls (measured at the kernel's launch)
 MAX_RANK = 256
 
 
@@ -45,13 +46,22 @@ class AdapterBatch:
                 run = [at, a, n]
                 tiles.append(run)
             at += n
-        tiles = [(t, min(TILE_TOKENS, t0 + n - t), a, 0) for t0, a, n in tiles if a >= 0
-                 for t in range(t0, t0 + n, TILE_TOKENS)]
-        self.n_tiles = len(tiles)
+        tiles = [[(t, min(size, t0 + n - t), a, 0) for t0, a, n in tiles if a >= 0 for t in range(t0, t0 + n, size)]
+                 for size in TILE_TOKENS]
         self.device = require_gfx950(device)
         self.token_adapter = upload(self.device, [a for n, a in zip(lengths, ids) for _ in range(n)])
-        self.tiles = upload(self.device, [x for t in tiles for x in t])
+        self.tiles = upload(self.device, [x for size in tiles for t in size for x in t])
+        self._lists = tuple(zip(TILE_TOKENS, map(len, tiles), (self.tiles.data_ptr(),
+                                                               self.tiles.data_ptr() + 16 * len(tiles[0]))))
+        self.any = bool(tiles[0])
         self._ready = Prepared(self.device, self.token_adapter, self.tiles)
+
+    def tile_list(self, rank):
+        """(address, tiles, tokens per tile at most) of the list for adapters of a rank."""
+        (small, n_small, at_small), (large, n_large, at_large) = self._lists
+        if n_small * (rank // 16) <= SMALL_PAIRS:
+            return at_small, n_small, small
+        return at_large, n_large, large
 
 
 class QKVAdapters:

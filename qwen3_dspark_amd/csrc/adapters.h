@@ -27,11 +27,11 @@ struct ShrinkArgs {
   const bf16* x;               // [T, hidden]
   const bf16* a;               // [adapters][3][rank][hidden]
   const float* scaling;        // [adapters]
-  const int32_t* tiles;        // [n_tiles][4]: first token, tokens (<= 16), adapter, 0
+  const int32_t* tiles;        // [n_tiles][4]: first token, tokens, adapter, 0
   bf16* u;                     // [3][T][2][rank]
   int tokens, hidden, adapters, rank, ranks;     // ranks: of which an adapter has its own
 };
-int launch_adapter_shrink(const ShrinkArgs& s, int n_tiles, hipStream_t stream);
+int launch_adapter_shrink(const ShrinkArgs& s, int n_tiles, int tile_tokens, hipStream_t stream);
 
 // Adds the adapters' part to the accumulators of TT x 32 tokens by 2 x 32 dims of one
 // wave (MFMA layout of head_gemm.h: row = dim, column = token).  acc(i, tt): the accumulator

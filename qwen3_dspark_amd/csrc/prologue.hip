@@ -253,13 +253,14 @@ extern "C" int dspark_qkv_prologue_adapted(const void* x, const void* wq, const 
                                            const int64_t* positions, const float* rope, int tokens, int hidden,
                                            float eps, const void* adapter_a, const void* adapter_b, const float* scaling,
                                            int adapters, int rank, int own_rank, const int32_t* token_adapter,
-                                           const int32_t* tiles, int n_tiles, void* u, void* q_out, void* k_out,
+                                           const int32_t* tiles, int n_tiles, int tile_tokens, void* u, void* q_out, void* k_out,
                                            void* v_out, int64_t kv_row_stride, void* stream) {
   clear_error();
   DSPARK_REQUIRE(adapter_a && adapter_b && scaling && token_adapter && tiles && u, "null pointer argument");
   DSPARK_REQUIRE(adapters >= 1 && adapter_rank(rank) && own_rank >= 1 && own_rank <= rank,
                  "need adapters >= 1, rank 16, 32 or a multiple of 64 up to 256 and own_rank in [1, rank]");
   DSPARK_REQUIRE(n_tiles >= 1, "n_tiles must be >= 1");
+  DSPARK_REQUIRE(tile_tokens == 16 || tile_tokens == 32, "tile_tokens must be 16 or 32");
   DSPARK_REQUIRE((((uintptr_t)adapter_a | (uintptr_t)adapter_b | (uintptr_t)u) & 15) == 0, "tensors must be 16-byte aligned");
   PrologueArgs a{};
   int rc = check_prologue(a, x, wq, wk, wv, q_norm, k_norm, inv_freq, positions, rope, tokens, hidden, eps, q_out, k_out,
@@ -267,7 +268,7 @@ extern "C" int dspark_qkv_prologue_adapted(const void* x, const void* wq, const 
   if (rc != OK) return rc;
   hipStream_t s = static_cast<hipStream_t>(stream);
   rc = launch_adapter_shrink(ShrinkArgs{a.x, static_cast<const bf16*>(adapter_a), scaling, tiles, static_cast<bf16*>(u),
-                                        tokens, hidden, adapters, rank, own_rank}, n_tiles, s);
+                                        tokens, hidden, adapters, rank, own_rank}, n_tiles, tile_tokens, s);
   if (rc != OK) return rc;
   const AdapterArgs ad{token_adapter, static_cast<const bf16*>(adapter_b), static_cast<const bf16*>(u), adapters, rank,
                        adapter_tile_tokens(tokens)};

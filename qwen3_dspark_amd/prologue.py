@@ -117,11 +117,11 @@ class QKVPrologue:
                  self.hidden, self.eps)
         into = (q.data_ptr(), outs[0].data_ptr(), outs[1].data_ptr(), KV_HEADS * HEAD_DIM,
                 _native.stream_handle(self.device))
-        if adapters is not None and batch.n_tiles:
+        if adapters is not None and batch.any:
             adapters.ready(batch, into[-1])
             scratch = torch.empty(adapters.scratch(t), dtype=torch.bfloat16, device=self.device)
             _native.call('dspark_qkv_prologue_adapted', *given, *adapters.pointers, batch.token_adapter.data_ptr(),
-                         batch.tiles.data_ptr(), batch.n_tiles, scratch.data_ptr(), *into)
+                         *batch.tile_list(adapters.padded_rank), scratch.data_ptr(), *into)
         else:
             _native.call('dspark_qkv_prologue', *given, *into)
         return q, outs[0], outs[1]

@@ -35,14 +35,14 @@ def test_entry_point_checks():
     def project(**kw):
         args = dict(x=fake, wq=fake, wk=fake, wv=fake, qn=fake, kn=fake, inv=fake, pos=fake, rope=None, tokens=4,
                     hidden=1024, eps=1e-6, a=fake, b=fake, scaling=fake, adapters=2, rank=16, own_rank=8, token=fake,
-                    tiles=fake, n_tiles=1, u=fake, q=fake, k=fake, v=fake, stride=1024, stream=None)
+                    tiles=fake, n_tiles=1, tile_tokens=16, u=fake, q=fake, k=fake, v=fake, stride=1024, stream=None)
         args.update(kw)
         return lib.dspark_qkv_prologue_adapted(*args.values()), lib.dspark_last_error().decode()
     off = ctypes.c_void_p(1 << 20 | 8)
     for kw, match in ((dict(x=None), 'null'), (dict(token=None), 'null'), (dict(u=None), 'null'), (dict(tiles=None), 'null'),
                       (dict(scaling=None), 'null'), (dict(adapters=0), 'adapters'), (dict(rank=24), 'rank'),
                       (dict(rank=48), 'rank'), (dict(rank=320), 'rank'), (dict(own_rank=17), 'own_rank'),
-                      (dict(own_rank=0), 'own_rank'), (dict(n_tiles=0), 'n_tiles'), (dict(tokens=0), 'tokens'),
+                      (dict(own_rank=0), 'own_rank'), (dict(n_tiles=0), 'n_tiles'), (dict(tile_tokens=24), 'tile_tokens'), (dict(tokens=0), 'tokens'),
                       (dict(hidden=64), 'hidden'), (dict(hidden=1000), 'hidden'), (dict(stride=1000), 'kv_row_stride'),
                       (dict(b=off), 'aligned'), (dict(u=off), 'aligned'), (dict(a=off), 'aligned'), (dict(x=off), 'aligned')):
         rc, message = project(**kw)

@@ -94,6 +94,18 @@ def test_high_ranks_of_many_tokens(tokens, rank):
     check(got, layer.expected(x, rope, lengths, [3, 0, -1, 1]))
 
 
+@pytest.mark.parametrize('pairs', [0, 10 ** 6])
+def test_tiles_of_both_sizes(pairs, monkeypatch):
+    from qwen3_dspark_amd import adapters
+    monkeypatch.setattr(adapters, 'SMALL_PAIRS', pairs)
+    layer = Layer(3, 33)
+    lengths, ids = [1, 16, 17, 31, 32, 33, 5, 100], [0, 1, 2, 0, 1, 2, -1, 0]
+    x, positions, rope = layer.inputs(sum(lengths))
+    got = layer.prologue(x, positions, rope=rope, adapters=layer.adapters,
+                         batch=adapters.AdapterBatch(DEV, lengths, ids))
+    check(got, layer.expected(x, rope, lengths, ids))
+
+
 @pytest.mark.parametrize('hidden,rank,adapters', [(128, 256, 2), (256, 3, 1), (2048, 64, 5)])
 def test_sizes(hidden, rank, adapters):
     from qwen3_dspark_amd.adapters import AdapterBatch
