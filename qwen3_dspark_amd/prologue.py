@@ -101,11 +101,11 @@ class QKVPrologue:
             if not isinstance(adapters, QKVAdapters):
                 raise ValueError('adapters must be a QKVAdapters')
             adapters.check(batch, t, self.hidden, self.device)
-        q = torch.empty((t, Q_HEADS, HEAD_DIM), dtype=torch.bfloat16, device=self.device)
+        q = hidden.new_empty((t, Q_HEADS, HEAD_DIM))
         outs = []
         for o in (k_out, v_out):
             if o is None:
-                o = torch.empty((t, KV_HEADS, HEAD_DIM), dtype=torch.bfloat16, device=self.device)
+                o = hidden.new_empty((t, KV_HEADS, HEAD_DIM))
             elif (o.dtype != torch.bfloat16 or o.device != self.device or o.shape[0] < t
                   or tuple(o.shape[1:]) != (KV_HEADS, HEAD_DIM) or o.stride(0) != KV_HEADS * HEAD_DIM
                   or o.stride(2) != 1 or o.stride(1) != HEAD_DIM):
@@ -119,7 +119,7 @@ class QKVPrologue:
                 _native.stream_handle(self.device))
         if adapters is not None and batch.any:
             adapters.ready(batch, into[-1])
-            scratch = torch.empty(adapters.scratch(t), dtype=torch.bfloat16, device=self.device)
+            scratch = hidden.new_empty(adapters.scratch(t))
             _native.call('dspark_qkv_prologue_adapted', *given, *adapters.pointers, batch.token_adapter.data_ptr(),
                          *batch.tile_list(adapters.padded_rank), scratch.data_ptr(), *into)
         else:

@@ -161,6 +161,8 @@ class LogitControls:
         self._bias_token = upload(self.device, tokens)
         self._bias_value = upload(self.device, values, torch.float64)
         self._ready = Prepared(self.device, self._penalties, self._bias_start, self._bias_token, self._bias_value)
+        self._rules = (self._penalties.data_ptr(), self._bias_start.data_ptr(), self._bias_token.data_ptr() or None,
+                       self._bias_value.data_ptr() or None)
         self._none, self._each = array('i', [0] * n), array('i', range(n))
 
     def __call__(self, logits, history, *, lengths, prompt_lengths=None, counts=None, tokens=None, slots=None,
@@ -214,7 +216,7 @@ class LogitControls:
                 or allowed.stride(1) != 1 or allowed.stride(0) < words):
             raise ValueError('allowed must be int32 [rows, ceil(vocab / 32)] with contiguous rows')
         if out is None:
-            out = torch.empty(logits.shape, dtype=logits.dtype, device=self.device)
+            out = logits.new_empty(logits.shape)
         elif (not isinstance(out, torch.Tensor) or out.shape != logits.shape or out.device != self.device
               or out.dtype not in (logits.dtype, torch.float32) or out.stride(1) != 1 or out.stride(0) < self.vocab):
             raise ValueError('out must be [rows, vocab] of the logits\' type or fp32, with contiguous rows')
@@ -229,11 +231,9 @@ class LogitControls:
         here = n <= _LAYOUT_ON_HOST
         place = layout.buffer_info()[0] if here else (layout := upload(self.device, layout)).data_ptr()
         fill = _LOWEST[out.dtype] if self.masked is None else self.masked
-        _native.call('dspark_logit_controls', logits.data_ptr(), dtype, logits.stride(0), self.vocab, place, here, n, rows, sum(lengths),
-                     history.data_ptr() or logits.data_ptr(), history.element_size(),
-                     history.stride(0), tokens.contiguous().data_ptr() if total else None, self._penalties.data_ptr(),
-                     self._bias_start.data_ptr(), self._bias_token.data_ptr() or None, self._bias_value.data_ptr() or None,
-                     None if allowed is None else allowed.data_ptr(), 0 if allowed is None else allowed.stride(0), fill,
+        _native.call('dspark_logit_controls', logits.data_ptr(), dtype, logits.stride(0), self.vocab, place, here, n, rows,
+                     sum(lengths), history.data_ptr() or logits.data_ptr(), history.element_size(), history.stride(0),
+                     tokens.contiguous().data_ptr() if total else None, *self._rules, None if allowed is None else allowed.data_ptr(), 0 if allowed is None else allowed.stride(0), fill,
                      out.data_ptr(), 0 if out.dtype == torch.bfloat16 else 1, out.stride(0), stream)
         return out
 
