@@ -1844,249 +1844,6 @@ __device__ __forceinline__ void prefill_merge(const VarlenArgs& a, const float* 
   }
 }
 
-// The prompt workgroup of list column `column` (COLUMNS), or of record `seg`, tile `t`.
-template <bool VERIFY, bool COLUMNS>
-__device__ __forceinline__ void prefill_workgroup(const VarlenArgs& a, unsigned char* smem, int column, int seg, int t) {
-  const int g = blockIdx.x & 7;
-  if (COLUMNS) {
-    const int32_t* pair = a.columns + 2 * column;
-    seg = min(__builtin_amdgcn_readfirstlane(pair[0]), a.n_work) - 1;
-    t = max(__builtin_amdgcn_readfirstlane(pair[1]), 0);
-  } else if (a.work) {
-    seg = a.n_work - 1 - seg;        // a plan puts its prompts after the runs, longest last
-  }
-  Segment sg;
-  if (COLUMNS || a.work) {
-    const int32_t* w = a.work + WORK_INTS * max(seg, 0);        // no record: no query tokens
-    sg = Segment{w[0], w[1], w[2], w[3], w[4], seg < 0 ? 0 : w[5], w[6], w[7]};
-  } else if (!chunk_segment(a, VERIFY, seg, sg)) {
-    return;
-  }
-  const int kl = __builtin_amdgcn_readfirstlane(sg.kl);
-  int ql = __builtin_amdgcn_readfirstlane(sg.ql);
-  if (!COLUMNS && plane_form(a, ql, kl)) ql = 0;               // the planes attend it
-  if (ql <= DECODE_TOKENS || PF_TOKENS * t >= ql) return;      // uniform across the workgroup
-  const int q0 = __builtin_amdgcn_readfirstlane(sg.q0);
-  const int k0 = __builtin_amdgcn_readfirstlane(sg.k0);
-  const int k1 = __builtin_amdgcn_readfirstlane(sg.k1);
-  const int start = __builtin_amdgcn_readfirstlane(sg.start);
-  const int pslot = __builtin_amdgcn_readfirstlane(sg.pslot);
-  const int n_tok = min(PF_TOKENS, ql - PF_TOKENS * t);
-  const int rg_log2 = n_tok <= PF_GROUP ? 0 : 1;
-  const int kg_count = PF_WAVES >> rg_log2;
-
-  const int lane = threadIdx.x & 63;
-  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  const int hh = lane >> 5;
-  const int n = lane & 31;
-  const int rg = wave & ((1 << rg_log2) - 1);
-  const int kg = wave >> rg_log2;
-  const int tok0 = PF_TOKENS * t + PF_GROUP * rg;       // the wave's first query token (below ql)
-  const int tok = tok0 + (n >> 1);
-  const bool row_ok = tok < ql;
-  // Keys visible to token x of the request, within this segment.
-  auto limit = [&](int x) { return min(k1, a.causal ? kl - ql + x + 1 : kl); };
-  const int kend = limit(min(PF_TOKENS * t + PF_TOKENS, ql) - 1);      // to any row of the workgroup
-  const int vis = row_ok ? limit(tok) : 0;
-  const int lim0 = limit(min(tok0 + 7, ql - 1));        // to any of the wave's first 8 tokens
-  const int hi = limit(min(tok0 + PF_GROUP, ql) - 1);   // to any row of the wave
-  const int full_lim = min(limit(tok0), hi);            // below: visible to every row
-
-  bf16x8 qf[8];
-  {
-    const bf16* qp = a.q + (size_t)(q0 + (row_ok ? tok : 0)) * Q_ROW + (size_t)(2 * g + (n & 1)) * HD + 8 * hh;
-    #pragma unroll
-    for (int ks = 0; ks < 8; ++ks) qf[ks] = ld8(qp + 16 * ks);
-  }
-
-  // Key j of the request: part A (committed rows) below a_len, else part B.
-  // Wave w loads rows 16w .. 16w+15 of a stage's K and V, 4 rows (1 KiB) per
-  // load: lane L of load i fetches row k = 16w + 4i + L/16 at 16-byte chunk
-  // (L%16) ^ swz(k).
-  const int a_len = VERIFY ? kl - ql : kl;
-  const int64_t b_stride = VERIFY ? KV_ROW : a.a_tok_stride;
-  const size_t abase = VERIFY ? (size_t)start * (size_t)a.slot_stride + (size_t)g * a.a_head_stride
-                              : (size_t)start * KV_ROW + (size_t)g * HD;
-  const size_t bbase = VERIFY ? (size_t)q0 * KV_ROW + (size_t)g * HD : abase;
-  const int row0 = 16 * wave;
-  const uint32_t col[2] = {(uint32_t)(16 * ((lane & 15) ^ swz(row0 + (lane >> 4)))),
-                           (uint32_t)(16 * ((lane & 15) ^ swz(row0 + 8 + (lane >> 4))))};
-  const uint32_t off_a = (uint32_t)((lane >> 4) * a.a_tok_stride * 2);
-  const uint32_t off_b = (uint32_t)((lane >> 4) * b_stride * 2);
-  const uint32_t smem_lds = lds_address(smem);
-  auto issue = [&](int step, bool is_v) {
-    const bf16* pa = (is_v ? a.v_a : a.k_a) + abase;
-    const bf16* pb = (is_v ? a.v_b : a.k_b) + bbase;
-    const uint32_t slot = smem_lds + (is_v ? PF_V : 0) + (uint32_t)((step & 1) * PF_HALF + wave * 4096);
-    const int kt = k0 + step * DSTEP;
-    const bool in_a = kt + DSTEP <= min(a_len, kend);
-    if (in_a || (kt >= a_len && kt + DSTEP <= kend)) {
-      // whole stage in one part: wave-uniform base plus per-lane offset
-      const int64_t stride = in_a ? a.a_tok_stride : b_stride;
-      const bf16* base = (in_a ? pa : pb) + (int64_t)(kt - (in_a ? 0 : a_len) + row0) * stride;
-      const uint32_t off = in_a ? off_a : off_b;
-      #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        lds_dma16_base(base + 4 * i * stride, off + col[i >> 1], __builtin_amdgcn_readfirstlane(slot + 1024u * i));
-    } else {
-      // rows clamped to the last visible key (masked out of the softmax)
-      #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int kk = min(kt + row0 + 4 * i + (lane >> 4), kend - 1);
-        const bf16* p = kk < a_len ? pa + (int64_t)kk * a.a_tok_stride : pb + (int64_t)(kk - a_len) * b_stride;
-        lds_dma16(reinterpret_cast<const char*>(p) + col[i >> 1], __builtin_amdgcn_readfirstlane(slot + 1024u * i));
-      }
-    }
-  };
-
-  PairState st;
-  st.m = -INFINITY;
-  st.l = 0.f;
-  #pragma unroll
-  for (int D = 0; D < 4; ++D) st.o[D] = f32x16{};
-  const TileOffsets co = ctx_tile_offsets<ROWB>(lane);
-  const int n_steps = kend > k0 ? (kend - k0 + DSTEP - 1) / DSTEP : 0;
-  if (n_steps > 0) {
-    issue(0, false);
-    issue(0, true);
-    if (n_steps > 1) issue(1, false);
-  }
-  // Q completes behind the first stage's loads (the compiler's wait for it
-  // drains them too), so that both round trips overlap.
-  settle(qf[0], qf[1], qf[2], qf[3], qf[4], qf[5], qf[6], qf[7]);
-  #pragma unroll
-  for (int ks = 0; ks < 8; ++ks) qf[ks] = row_ok ? qf[ks] : zero8();
-  settle(qf[0], qf[1], qf[2], qf[3], qf[4], qf[5], qf[6], qf[7]);
-
-  // Half stage 2s + h goes to key group (2s + h) mod kg_count.  Step s takes
-  // V of stage s and forms the scores of stage s + 1, one stage ahead; it
-  // begins once both have landed for every wave (and every wave's LDS reads of
-  // the step before are done), and starts the loads of the next step.
-  const int h = kg & 1;
-  auto turn = [&](int s) { return ((2 * s) & (kg_count - 1)) == (kg & ~1); };
-  auto key0 = [&](int s) { return k0 + s * DSTEP + 32 * h; };
-  auto k_at = [&](int s) { return smem_lds + (uint32_t)((s & 1) * PF_HALF + 32 * h * ROWB) + co.k; };
-  auto v_at = [&](int s) { return smem_lds + (uint32_t)(PF_V + (s & 1) * PF_HALF + 32 * h * ROWB) + co.v; };
-  auto arrive = [&]() {
-    // not before the MFMAs of the step that ends here, which hide the loads
-    __builtin_amdgcn_sched_barrier(0);
-    load_wait<0>();
-    ring_barrier();
-  };
-  auto enter = [&](int s) {
-    arrive();
-    if (s + 1 < n_steps) issue(s + 1, true);
-    if (s + 2 < n_steps) issue(s + 2, false);
-  };
-  // Scores of the next stage; past the last stage they are of stale rows and
-  // never used.
-  auto ahead = [&](int s) {
-    bf16x8 kf[8];
-    prefill_k(kf, k_at(s));
-    return prefill_scores(qf, kf);
-  };
-  f32x16 x = {};
-  int s = 0;
-  if (n_steps > 0) {
-    arrive();
-    if (turn(0)) x = ahead(0);
-  }
-  if (kg_count == 2) {
-    // One tile per stage and wave: those below every row's limit first, two
-    // per iteration (no copies of the scores).  The waves of a workgroup may
-    // differ in how many these are; every wave passes one barrier per step.
-    const int span = max(0, full_lim - k0 - 32 * h);
-    const int full = span / DSTEP + (span % DSTEP >= 32 ? 1 : 0);
-    for (; s + 1 < full; s += 2) {
-      enter(s);
-      const f32x16 y = prefill_full_tile(st, qf, x, k_at(s + 1), v_at(s), a.scale_log2);
-      enter(s + 1);
-      x = prefill_full_tile(st, qf, y, k_at(s + 2), v_at(s + 1), a.scale_log2);
-    }
-    if (s < full) {
-      enter(s);
-      x = prefill_full_tile(st, qf, x, k_at(s + 1), v_at(s), a.scale_log2);
-      ++s;
-    }
-  }
-  for (; s < n_steps; ++s) {
-    enter(s);
-    if (turn(s) && key0(s) < hi) {
-      const int kt = key0(s);
-      if (kt + 32 > full_lim) {
-        prefill_edge_tile(st, x, v_at(s), vis - kt - 8 * hh, lim0 - kt, hi - kt, a.scale_log2);
-      } else {
-        const float m_use = prefill_max(st, x, a.scale_log2);
-        bf16x8 ph[2], pl[2];
-        prefill_probs(st, x, m_use, a.scale_log2, ph, pl);
-        #pragma unroll
-        for (int u = 0; u < 2; ++u)
-          #pragma unroll
-          for (int D = 0; D < 4; ++D) {
-            const bf16x8 v = prefill_v(v_at(s), u, D);
-            st.o[D] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v, ph[u], st.o[D], 0, 0, 0);
-            st.o[D] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v, pl[u], st.o[D], 0, 0, 0);
-          }
-      }
-    }
-    if (turn(s + 1)) x = ahead(s + 1);
-  }
-  __syncthreads();   // every wave is done with the stages
-
-  // The key groups' states merge with the online-softmax rule: every wave
-  // leaves its state in LDS, then folds and writes its share of the dims.
-  float* mb = reinterpret_cast<float*>(smem + wave * PF_STATE);
-  #pragma unroll
-  for (int D = 0; D < 4; ++D)
-    #pragma unroll
-    for (int q = 0; q < 4; ++q)
-      *reinterpret_cast<f32x4*>(mb + ((4 * D + q) * WAVE + lane) * 4) =
-          f32x4{st.o[D][4 * q], st.o[D][4 * q + 1], st.o[D][4 * q + 2], st.o[D][4 * q + 3]};
-  mb[64 * WAVE + lane] = st.m;
-  mb[65 * WAVE + lane] = st.l;
-  __syncthreads();
-  const float* group = reinterpret_cast<const float*>(smem + rg * PF_STATE);
-  if (kg_count == 2) prefill_merge<2>(a, group, 2 * PF_STATE / 4, kg, q0, tok, ql, g, n, hh, pslot);
-  else prefill_merge<4>(a, group, PF_STATE / 4, kg, q0, tok, ql, g, n, hh, pslot);
-  // Fused stage: the workgroups of the request's last segment copy their own
-  // tokens' new rows of KV head g into the scratch layer.
-  if (VERIFY && a.stage_k && k1 == kl) {
-    const int half = 16 * n_tok;
-    for (int i = threadIdx.x; i < 2 * half; i += PF_WAVES * WAVE) {
-      const bool vh = i >= half;
-      const int rem = vh ? i - half : i;
-      const size_t off = bbase + (size_t)(PF_TOKENS * t + (rem >> 4)) * KV_ROW + (size_t)(rem & 15) * 8;
-      *reinterpret_cast<bf16x8*>((vh ? a.stage_v : a.stage_k) + off) = ld8((vh ? a.v_b : a.k_b) + off);
-    }
-  }
-}
-
-// A call whose max_q exceeds DECODE_TOKENS is one launch: first the workgroups that
-// walk the runs, then the prompts'.  With COLUMNS (a mixed plan) those are the listed
-// (record, tile) pairs, in the order of the list, which starts with the longest; else
-// the grid is gridDim.x = 8 x the tiles of max_q wide, its first `decode_rows` rows
-// walk the runs (or fixed chunks), a plane after the other, and one row follows per
-// record: each request is then attended by one of the two forms by its own lengths.
-template <bool VERIFY, bool COLUMNS>
-__global__ __launch_bounds__(PF_WAVES * WAVE, 2) void prefill_attn_kernel(VarlenArgs a, int decode_grid, int decode_rows) {
-  // 1 KiB alignment: tile offsets are XORed into LDS addresses.
-  __shared__ __attribute__((aligned(1024))) unsigned char smem[PF_SMEM];
-  static_assert(PF_SMEM >= VARLEN_SMEM && PF_WAVES * WAVE == 256, "one launch shape for both forms");
-  const int row = blockIdx.y + PF_SEGS_Y * blockIdx.z;
-  const int wid = (int)(blockIdx.x + gridDim.x * (unsigned)row);        // keeps the XCD: gridDim.x is a multiple of 8
-  if (COLUMNS ? wid < decode_grid : row < decode_rows) {
-    if (COLUMNS) {
-      varlen_workgroup<VERIFY, true, RECORDS>(a, smem, wid, decode_grid, 0);
-    } else {
-      const int plane = wid / decode_grid;
-      if (plane < a.planes) varlen_workgroup<VERIFY, true, PLANES>(a, smem, wid - plane * decode_grid, decode_grid, plane);
-    }
-    return;
-  }
-  prefill_workgroup<VERIFY, COLUMNS>(a, smem, (wid - decode_grid) >> 3, row - decode_rows,
-                                     (int)(gridDim.x >> 3) - 1 - (int)(blockIdx.x >> 3));
-}
-
 // ---------------------------------------------------------------------------
 // A prefix that many requests of a verification batch share (the same committed rows, of
 // which each keeps a copy): attended once for all of them
@@ -2103,8 +1860,9 @@ __global__ __launch_bounds__(PF_WAVES * WAVE, 2) void prefill_attn_kernel(Varlen
 // head blockIdx.x % 8, whose keys its XCD's L2 then holds for all of the group's token
 // tiles; the grid is fixed and the list says how many items there are, so that a captured
 // launch serves every transaction.  Tiles and stages as in prefill_attn_kernel.  The items
-// go in the launch of the requests' own keys: in a launch of their own, 16 requests x 7 tokens
-// over 2,048 shared rows 25.5 us a call, together 20.4, 64 over 8,192 75 / 55.
+// go in the launch of the requests' own keys: from launches of their own 16 requests x 7 tokens
+// over 2,000 shared rows came from 25.5 to 20.4 us a call, 64 over 8,192 from 74.7 to 55, 7 of
+// which are the single operand of prefix_probs.
 //
 // Bound by the vector unit, then the matrix unit: 12 prompts of 2,645 tokens over two
 // prefixes of 5,379 and 6,000 rows (126 GFLOP) take 166 to 192 us, 0.65 to 0.75 PFLOP/s, in which vector instructions issue
@@ -2345,25 +2103,275 @@ __device__ __forceinline__ void prefix_workgroup(const PrefixArgs& a, unsigned c
   }
 }
 
-// One launch for all parts of a batch: `members` x 8 workgroups walk the prefix items,
-// `runs` x 8 the runs of the requests' own keys, then one follows per (prompt column, KV
-// head).  The first two are dealt in turns of `turn` columns, a CU's worth each, so that a CU
-// has one of either: the prefix's are bound by the matrix units, the runs by memory.
-template <bool COLUMNS>
-__global__ __launch_bounds__(PF_WAVES * WAVE, 2) void shared_attn_kernel(VarlenArgs a, PrefixArgs p, int members, int runs,
-                                                                         int turn) {
+// The first workgroups of a launch with shared prefixes: `members` x 8 walk the prefix items,
+// `runs` x 8 the runs of the requests' own keys.  They are dealt in turns of `turn` columns of
+// 8, a CU's worth each, so that a CU has one of either: the prefix's are bound by the vector and
+// matrix units, the runs by memory.
+struct NoPrefix {
+  static constexpr bool ANY = false;
+};
+struct SharedArgs {
+  static constexpr bool ANY = true;
+  PrefixArgs prefix;
+  int members, runs, turn;
+};
+template <bool PROMPTS>
+__device__ __forceinline__ void shared_workgroup(const VarlenArgs& a, const SharedArgs& s, unsigned char* smem, int wid) {
+  const int c = wid >> 3;
+  const int both = min(s.members, s.runs) / s.turn * s.turn;     // of either, in turns
+  const int round = c / (2 * s.turn), at = c % (2 * s.turn);
+  const bool prefix = c < 2 * both ? at < s.turn : c - 2 * both < s.members - both;
+  const int i = c < 2 * both ? round * s.turn + at % s.turn : prefix ? c - both : c - s.members;
+  if (prefix) prefix_workgroup(s.prefix, smem, i, s.members);
+  else varlen_workgroup<true, PROMPTS, RECORDS>(a, smem, 8 * i + (wid & 7), 8 * s.runs, 0);
+}
+
+// A batch with shared prefixes and no prompts; with prompts prefill_attn_kernel is the launch.
+__global__ __launch_bounds__(PF_WAVES * WAVE, 2) void shared_attn_kernel(VarlenArgs a, SharedArgs shared) {
   __shared__ __attribute__((aligned(1024))) unsigned char smem[PF_SMEM];
-  const int c = blockIdx.x >> 3;
-  if (c >= members + runs) {
-    if constexpr (COLUMNS) prefill_workgroup<true, true>(a, smem, c - members - runs, 0, 0);
+  shared_workgroup<false>(a, shared, smem, blockIdx.x);
+}
+
+// A call whose max_q exceeds DECODE_TOKENS is one launch: first the workgroups that
+// walk the runs, then the prompts'.  With COLUMNS (a mixed plan) those are the listed
+// (record, tile) pairs, in the order of the list, which starts with the longest; else
+// the grid is gridDim.x = 8 x the tiles of max_q wide, its first `decode_rows` rows
+// walk the runs (or fixed chunks), a plane after the other, and one row follows per
+// record: each request is then attended by one of the two forms by its own lengths.
+// With PREFIX (SharedArgs) the first workgroups walk the items of shared prefixes too.
+template <bool VERIFY, bool COLUMNS, class PREFIX = NoPrefix>
+__global__ __launch_bounds__(PF_WAVES * WAVE, 2) void prefill_attn_kernel(VarlenArgs a, int decode_grid, int decode_rows,
+                                                                         PREFIX shared) {
+  // 1 KiB alignment: tile offsets are XORed into LDS addresses.
+  __shared__ __attribute__((aligned(1024))) unsigned char smem[PF_SMEM];
+  static_assert(PF_SMEM >= VARLEN_SMEM && PF_WAVES * WAVE == 256, "one launch shape for both forms");
+  const int row = blockIdx.y + PF_SEGS_Y * blockIdx.z;
+  const int wid = (int)(blockIdx.x + gridDim.x * (unsigned)row);        // keeps the XCD: gridDim.x is a multiple of 8
+  if (COLUMNS ? wid < decode_grid : row < decode_rows) {
+    if constexpr (PREFIX::ANY) {
+      shared_workgroup<true>(a, shared, smem, wid);
+    } else if (COLUMNS) {
+      varlen_workgroup<VERIFY, true, RECORDS>(a, smem, wid, decode_grid, 0);
+    } else {
+      const int plane = wid / decode_grid;
+      if (plane < a.planes) varlen_workgroup<VERIFY, true, PLANES>(a, smem, wid - plane * decode_grid, decode_grid, plane);
+    }
     return;
   }
-  const int both = min(members, runs) / turn * turn;             // of either, in turns
-  const int round = c / (2 * turn), at = c % (2 * turn);
-  const bool prefix = c < 2 * both ? at < turn : c - 2 * both < members - both;
-  const int i = c < 2 * both ? round * turn + at % turn : prefix ? c - both : c - members;
-  if (prefix) prefix_workgroup(p, smem, i, members);
-  else varlen_workgroup<true, COLUMNS, RECORDS>(a, smem, 8 * i + (blockIdx.x & 7), 8 * runs, 0);
+  const int g = blockIdx.x & 7;
+  int t = (gridDim.x >> 3) - 1 - (blockIdx.x >> 3);
+  int seg = row - decode_rows;
+  if (COLUMNS) {
+    const int32_t* column = a.columns + 2 * ((wid - decode_grid) >> 3);
+    seg = min(__builtin_amdgcn_readfirstlane(column[0]), a.n_work) - 1;
+    t = max(__builtin_amdgcn_readfirstlane(column[1]), 0);
+  } else if (a.work) {
+    seg = a.n_work - 1 - seg;        // a plan puts its prompts after the runs, longest last
+  }
+  Segment sg;
+  if (COLUMNS || a.work) {
+    const int32_t* w = a.work + WORK_INTS * max(seg, 0);        // no record: no query tokens
+    sg = Segment{w[0], w[1], w[2], w[3], w[4], seg < 0 ? 0 : w[5], w[6], w[7]};
+  } else if (!chunk_segment(a, VERIFY, seg, sg)) {
+    return;
+  }
+  const int kl = __builtin_amdgcn_readfirstlane(sg.kl);
+  int ql = __builtin_amdgcn_readfirstlane(sg.ql);
+  if (!COLUMNS && plane_form(a, ql, kl)) ql = 0;               // the planes attend it
+  if (ql <= DECODE_TOKENS || PF_TOKENS * t >= ql) return;      // uniform across the workgroup
+  const int q0 = __builtin_amdgcn_readfirstlane(sg.q0);
+  const int k0 = __builtin_amdgcn_readfirstlane(sg.k0);
+  const int k1 = __builtin_amdgcn_readfirstlane(sg.k1);
+  const int start = __builtin_amdgcn_readfirstlane(sg.start);
+  const int pslot = __builtin_amdgcn_readfirstlane(sg.pslot);
+  const int n_tok = min(PF_TOKENS, ql - PF_TOKENS * t);
+  const int rg_log2 = n_tok <= PF_GROUP ? 0 : 1;
+  const int kg_count = PF_WAVES >> rg_log2;
+
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int hh = lane >> 5;
+  const int n = lane & 31;
+  const int rg = wave & ((1 << rg_log2) - 1);
+  const int kg = wave >> rg_log2;
+  const int tok0 = PF_TOKENS * t + PF_GROUP * rg;       // the wave's first query token (below ql)
+  const int tok = tok0 + (n >> 1);
+  const bool row_ok = tok < ql;
+  // Keys visible to token x of the request, within this segment.
+  auto limit = [&](int x) { return min(k1, a.causal ? kl - ql + x + 1 : kl); };
+  const int kend = limit(min(PF_TOKENS * t + PF_TOKENS, ql) - 1);      // to any row of the workgroup
+  const int vis = row_ok ? limit(tok) : 0;
+  const int lim0 = limit(min(tok0 + 7, ql - 1));        // to any of the wave's first 8 tokens
+  const int hi = limit(min(tok0 + PF_GROUP, ql) - 1);   // to any row of the wave
+  const int full_lim = min(limit(tok0), hi);            // below: visible to every row
+
+  bf16x8 qf[8];
+  {
+    const bf16* qp = a.q + (size_t)(q0 + (row_ok ? tok : 0)) * Q_ROW + (size_t)(2 * g + (n & 1)) * HD + 8 * hh;
+    #pragma unroll
+    for (int ks = 0; ks < 8; ++ks) qf[ks] = ld8(qp + 16 * ks);
+  }
+
+  // Key j of the request: part A (committed rows) below a_len, else part B.
+  // Wave w loads rows 16w .. 16w+15 of a stage's K and V, 4 rows (1 KiB) per
+  // load: lane L of load i fetches row k = 16w + 4i + L/16 at 16-byte chunk
+  // (L%16) ^ swz(k).
+  const int a_len = VERIFY ? kl - ql : kl;
+  const int64_t b_stride = VERIFY ? KV_ROW : a.a_tok_stride;
+  const size_t abase = VERIFY ? (size_t)start * (size_t)a.slot_stride + (size_t)g * a.a_head_stride
+                              : (size_t)start * KV_ROW + (size_t)g * HD;
+  const size_t bbase = VERIFY ? (size_t)q0 * KV_ROW + (size_t)g * HD : abase;
+  const int row0 = 16 * wave;
+  const uint32_t col[2] = {(uint32_t)(16 * ((lane & 15) ^ swz(row0 + (lane >> 4)))),
+                           (uint32_t)(16 * ((lane & 15) ^ swz(row0 + 8 + (lane >> 4))))};
+  const uint32_t off_a = (uint32_t)((lane >> 4) * a.a_tok_stride * 2);
+  const uint32_t off_b = (uint32_t)((lane >> 4) * b_stride * 2);
+  const uint32_t smem_lds = lds_address(smem);
+  auto issue = [&](int step, bool is_v) {
+    const bf16* pa = (is_v ? a.v_a : a.k_a) + abase;
+    const bf16* pb = (is_v ? a.v_b : a.k_b) + bbase;
+    const uint32_t slot = smem_lds + (is_v ? PF_V : 0) + (uint32_t)((step & 1) * PF_HALF + wave * 4096);
+    const int kt = k0 + step * DSTEP;
+    const bool in_a = kt + DSTEP <= min(a_len, kend);
+    if (in_a || (kt >= a_len && kt + DSTEP <= kend)) {
+      // whole stage in one part: wave-uniform base plus per-lane offset
+      const int64_t stride = in_a ? a.a_tok_stride : b_stride;
+      const bf16* base = (in_a ? pa : pb) + (int64_t)(kt - (in_a ? 0 : a_len) + row0) * stride;
+      const uint32_t off = in_a ? off_a : off_b;
+      #pragma unroll
+      for (int i = 0; i < 4; ++i)
+        lds_dma16_base(base + 4 * i * stride, off + col[i >> 1], __builtin_amdgcn_readfirstlane(slot + 1024u * i));
+    } else {
+      // rows clamped to the last visible key (masked out of the softmax)
+      #pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int kk = min(kt + row0 + 4 * i + (lane >> 4), kend - 1);
+        const bf16* p = kk < a_len ? pa + (int64_t)kk * a.a_tok_stride : pb + (int64_t)(kk - a_len) * b_stride;
+        lds_dma16(reinterpret_cast<const char*>(p) + col[i >> 1], __builtin_amdgcn_readfirstlane(slot + 1024u * i));
+      }
+    }
+  };
+
+  PairState st;
+  st.m = -INFINITY;
+  st.l = 0.f;
+  #pragma unroll
+  for (int D = 0; D < 4; ++D) st.o[D] = f32x16{};
+  const TileOffsets co = ctx_tile_offsets<ROWB>(lane);
+  const int n_steps = kend > k0 ? (kend - k0 + DSTEP - 1) / DSTEP : 0;
+  if (n_steps > 0) {
+    issue(0, false);
+    issue(0, true);
+    if (n_steps > 1) issue(1, false);
+  }
+  // Q completes behind the first stage's loads (the compiler's wait for it
+  // drains them too), so that both round trips overlap.
+  settle(qf[0], qf[1], qf[2], qf[3], qf[4], qf[5], qf[6], qf[7]);
+  #pragma unroll
+  for (int ks = 0; ks < 8; ++ks) qf[ks] = row_ok ? qf[ks] : zero8();
+  settle(qf[0], qf[1], qf[2], qf[3], qf[4], qf[5], qf[6], qf[7]);
+
+  // Half stage 2s + h goes to key group (2s + h) mod kg_count.  Step s takes
+  // V of stage s and forms the scores of stage s + 1, one stage ahead; it
+  // begins once both have landed for every wave (and every wave's LDS reads of
+  // the step before are done), and starts the loads of the next step.
+  const int h = kg & 1;
+  auto turn = [&](int s) { return ((2 * s) & (kg_count - 1)) == (kg & ~1); };
+  auto key0 = [&](int s) { return k0 + s * DSTEP + 32 * h; };
+  auto k_at = [&](int s) { return smem_lds + (uint32_t)((s & 1) * PF_HALF + 32 * h * ROWB) + co.k; };
+  auto v_at = [&](int s) { return smem_lds + (uint32_t)(PF_V + (s & 1) * PF_HALF + 32 * h * ROWB) + co.v; };
+  auto arrive = [&]() {
+    // not before the MFMAs of the step that ends here, which hide the loads
+    __builtin_amdgcn_sched_barrier(0);
+    load_wait<0>();
+    ring_barrier();
+  };
+  auto enter = [&](int s) {
+    arrive();
+    if (s + 1 < n_steps) issue(s + 1, true);
+    if (s + 2 < n_steps) issue(s + 2, false);
+  };
+  // Scores of the next stage; past the last stage they are of stale rows and
+  // never used.
+  auto ahead = [&](int s) {
+    bf16x8 kf[8];
+    prefill_k(kf, k_at(s));
+    return prefill_scores(qf, kf);
+  };
+  f32x16 x = {};
+  int s = 0;
+  if (n_steps > 0) {
+    arrive();
+    if (turn(0)) x = ahead(0);
+  }
+  if (kg_count == 2) {
+    // One tile per stage and wave: those below every row's limit first, two
+    // per iteration (no copies of the scores).  The waves of a workgroup may
+    // differ in how many these are; every wave passes one barrier per step.
+    const int span = max(0, full_lim - k0 - 32 * h);
+    const int full = span / DSTEP + (span % DSTEP >= 32 ? 1 : 0);
+    for (; s + 1 < full; s += 2) {
+      enter(s);
+      const f32x16 y = prefill_full_tile(st, qf, x, k_at(s + 1), v_at(s), a.scale_log2);
+      enter(s + 1);
+      x = prefill_full_tile(st, qf, y, k_at(s + 2), v_at(s + 1), a.scale_log2);
+    }
+    if (s < full) {
+      enter(s);
+      x = prefill_full_tile(st, qf, x, k_at(s + 1), v_at(s), a.scale_log2);
+      ++s;
+    }
+  }
+  for (; s < n_steps; ++s) {
+    enter(s);
+    if (turn(s) && key0(s) < hi) {
+      const int kt = key0(s);
+      if (kt + 32 > full_lim) {
+        prefill_edge_tile(st, x, v_at(s), vis - kt - 8 * hh, lim0 - kt, hi - kt, a.scale_log2);
+      } else {
+        const float m_use = prefill_max(st, x, a.scale_log2);
+        bf16x8 ph[2], pl[2];
+        prefill_probs(st, x, m_use, a.scale_log2, ph, pl);
+        #pragma unroll
+        for (int u = 0; u < 2; ++u)
+          #pragma unroll
+          for (int D = 0; D < 4; ++D) {
+            const bf16x8 v = prefill_v(v_at(s), u, D);
+            st.o[D] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v, ph[u], st.o[D], 0, 0, 0);
+            st.o[D] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v, pl[u], st.o[D], 0, 0, 0);
+          }
+      }
+    }
+    if (turn(s + 1)) x = ahead(s + 1);
+  }
+  __syncthreads();   // every wave is done with the stages
+
+  // The key groups' states merge with the online-softmax rule: every wave
+  // leaves its state in LDS, then folds and writes its share of the dims.
+  float* mb = reinterpret_cast<float*>(smem + wave * PF_STATE);
+  #pragma unroll
+  for (int D = 0; D < 4; ++D)
+    #pragma unroll
+    for (int q = 0; q < 4; ++q)
+      *reinterpret_cast<f32x4*>(mb + ((4 * D + q) * WAVE + lane) * 4) =
+          f32x4{st.o[D][4 * q], st.o[D][4 * q + 1], st.o[D][4 * q + 2], st.o[D][4 * q + 3]};
+  mb[64 * WAVE + lane] = st.m;
+  mb[65 * WAVE + lane] = st.l;
+  __syncthreads();
+  const float* group = reinterpret_cast<const float*>(smem + rg * PF_STATE);
+  if (kg_count == 2) prefill_merge<2>(a, group, 2 * PF_STATE / 4, kg, q0, tok, ql, g, n, hh, pslot);
+  else prefill_merge<4>(a, group, PF_STATE / 4, kg, q0, tok, ql, g, n, hh, pslot);
+  // Fused stage: the workgroups of the request's last segment copy their own
+  // tokens' new rows of KV head g into the scratch layer.
+  if (VERIFY && a.stage_k && k1 == kl) {
+    const int half = 16 * n_tok;
+    for (int i = threadIdx.x; i < 2 * half; i += PF_WAVES * WAVE) {
+      const bool vh = i >= half;
+      const int rem = vh ? i - half : i;
+      const size_t off = bbase + (size_t)(PF_TOKENS * t + (rem >> 4)) * KV_ROW + (size_t)(rem & 15) * 8;
+      *reinterpret_cast<bf16x8*>((vh ? a.stage_v : a.stage_k) + off) = ld8((vh ? a.v_b : a.k_b) + off);
+    }
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -2519,7 +2527,7 @@ int launch_prefill(const VarlenArgs& a, unsigned grid, unsigned prompts, int max
   const unsigned decode_rows = (grid * a.planes + gx - 1) / gx;
   const unsigned rows = decode_rows + prompts;
   hipLaunchKernelGGL((prefill_attn_kernel<VERIFY, false>), dim3(gx, std::min(rows, (unsigned)PF_SEGS_Y), (rows + PF_SEGS_Y - 1) / PF_SEGS_Y),
-                     dim3(256), 0, s, a, (int)grid, (int)decode_rows);
+                     dim3(256), 0, s, a, (int)grid, (int)decode_rows, NoPrefix{});
   return launch_status("prefill_attn_kernel");
 }
 
@@ -2710,7 +2718,7 @@ extern "C" int dspark_mixed_attn_fwd(const void* q, const void* k, const void* v
   } else {
     a.columns = requests + REQ_INTS * n_req;
     hipLaunchKernelGGL((verify ? prefill_attn_kernel<true, true> : prefill_attn_kernel<false, true>),
-                       dim3(grid + (unsigned)n_columns * HKV), dim3(256), 0, s, a, (int)grid, 0);
+                       dim3(grid + (unsigned)n_columns * HKV), dim3(256), 0, s, a, (int)grid, 0, NoPrefix{});
     rc = launch_status("prefill_attn_kernel");
   }
   if (rc != OK || part_tiles == 0) return rc;
@@ -2771,12 +2779,15 @@ extern "C" int dspark_shared_attn_fwd(const void* q, int64_t q_rows, const void*
   a.scale_log2 = scale * LOG2E;
   const int32_t* requests = work + WORK_INTS * n_work + n_groups + 1;
   a.columns = requests + REQ_INTS * n_req;
-  const PrefixArgs p{a.q, a.k_a, a.v_a, slot_stride, tok_stride, head_stride, prefixes, a.part_o, a.part_ml, max_items,
-                     max_tokens, part_tiles, (int)q_rows, a.scale_log2};
+  const SharedArgs shared{{a.q, a.k_a, a.v_a, slot_stride, tok_stride, head_stride, prefixes, a.part_o, a.part_ml, max_items,
+                           max_tokens, part_tiles, (int)q_rows, a.scale_log2}, members, n_groups, turn};
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const dim3 grid((unsigned)(members + n_groups + n_columns) * HKV);
-  hipLaunchKernelGGL((n_columns ? shared_attn_kernel<true> : shared_attn_kernel<false>), grid, dim3(PF_WAVES * WAVE), 0, s, a,
-                     p, members, n_groups, turn);
+  const int first = (members + n_groups) * HKV;
+  if (n_columns)
+    hipLaunchKernelGGL((prefill_attn_kernel<true, true, SharedArgs>), dim3((unsigned)(first + n_columns * HKV)),
+                       dim3(PF_WAVES * WAVE), 0, s, a, first, 0, shared);
+  else
+    hipLaunchKernelGGL(shared_attn_kernel, dim3((unsigned)first), dim3(PF_WAVES * WAVE), 0, s, a, shared);
   rc = launch_status("shared_attn_kernel");
   if (rc != OK) return rc;
   MergeArgs m{requests, nullptr, nullptr, nullptr, nullptr, a.part_o, a.part_ml, a.out, n_req, 0, 0, 0};
