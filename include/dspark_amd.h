@@ -229,7 +229,8 @@ int dspark_mixed_attn_fwd(const void* q, const void* k, const void* v, const voi
  * members workgroups per KV head walk the items; they and the runs are dealt to the CUs in
  * turns of `turn` (a CU per KV head and column: the CU count / 8).  Lists of any length up
  * to the bounds, empty ones too, launch alike, so that a captured call serves lists to
- * come.  workspace: dspark_attn_workspace_bytes(part_tiles, 0, 1, 32) bytes.
+ * come.  tok_stride: at most 2^28.  workspace: dspark_attn_workspace_bytes(part_tiles, 0, 1, 32)
+ * bytes.
  */
 int dspark_shared_attn_fwd(const void* q, int64_t q_rows, const void* k_res, const void* v_res, const void* k_new,
                            const void* v_new, void* k_scr, void* v_scr, int n_req, int64_t slot_stride,

@@ -33,7 +33,7 @@ class AdapterBatch:
     def __init__(self, device, lengths, ids):
         lengths, ids = list(lengths), list(ids)
         if (not lengths or len(lengths) != len(ids) or any(type(n) is not int or n < 1 for n in lengths)
-                or any(type(a) is not int or a < -1 for a in ids)):
+                or any(type(a) is not int or not -1 <= a < 2 ** 31 for a in ids)):
             raise ValueError('One positive length and one adapter (or -1) per request required')
         self.tokens, self.largest = sum(lengths), max(ids)
         if self.tokens >= 2 ** 31:

@@ -9,7 +9,7 @@ from qwen3_dspark_amd.adapters import AdapterBatch, QKVAdapters
 
 
 @pytest.mark.parametrize('lengths,ids', [([], []), ([1], []), ([0], [0]), ([2, -1], [0, 0]), ([1], [-2]), ([1.5], [0]),
-                                         ([1], [None]), ([True], [0])])
+                                         ([1], [None]), ([True], [0]), ([1], [2 ** 31])])
 def test_batches_are_checked_before_the_device(lengths, ids):
     with pytest.raises(ValueError, match='One positive length'):
         AdapterBatch('cpu', lengths, ids)

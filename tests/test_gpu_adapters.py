@@ -211,6 +211,18 @@ def test_prepared_on_a_busy_stream():
         check(g, want)
 
 
+@pytest.mark.parametrize('tokens', [3, 300, 600])
+def test_rows_behind_the_batch_stay(tokens):
+    from qwen3_dspark_amd.adapters import AdapterBatch
+    layer = Layer(2, 16)
+    x, positions, rope = layer.inputs(tokens)
+    k, v = (torch.full((tokens + 200, 8, D), 3.0, dtype=torch.bfloat16, device=DEV) for _ in 'kv')
+    batch = AdapterBatch(DEV, [1, tokens - 1], [1, 0])
+    q, _, _ = layer.prologue(x, positions, k_out=k, v_out=v, rope=rope, adapters=layer.adapters, batch=batch)
+    check((q, k[:tokens], v[:tokens]), layer.expected(x, rope, [1, tokens - 1], [1, 0]))
+    assert (k[tokens:] == 3).all() and (v[tokens:] == 3).all()
+
+
 def test_staged_in_a_transaction():
     from qwen3_dspark_amd.adapters import AdapterBatch
     from qwen3_dspark_amd.persistent_kv import Bucket, PersistentTargetKV

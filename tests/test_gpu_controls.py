@@ -119,6 +119,24 @@ def test_texts_that_are_long_for_their_rows(vocab, pad, mask, dtype, out):
     check(b.call(out=o), b.expected(), b.out_dtype)
 
 
+def test_far_rows():
+    """Rows of logits, output, text and masks behind 2^31 elements."""
+    b = Batch(700, [1, 0], 40, torch.bfloat16, seed=11)
+    words, step = 22, 2 ** 30 + 8
+
+    def far(x):
+        out = torch.empty(2 * step + x.shape[1], dtype=x.dtype, device=DEV).as_strided(x.shape, (step, 1))
+        return out.copy_(x)
+    b.history = torch.cat((b.history, b.history[:1]))             # the third row is the second request's text
+    kw = dict(lengths=b.lengths, prompt_lengths=b.prompts, counts=b.counts, tokens=b.proposed, slots=[0, 2])
+    b.lengths[1] = kw['lengths'][1] = b.lengths[0]
+    b.prompts[1] = kw['prompt_lengths'][1] = b.prompts[0]
+    got = b.controls()(far(b.logits), far(b.history), allowed=far(pack(b.allowed, words)), out=far(b.logits), **kw)
+    check(got, b.expected(slots=[0, 2]), torch.bfloat16)
+    del got
+    torch.cuda.empty_cache()
+
+
 def test_many_requests():
     """More than a launch's arguments hold: the layout is uploaded."""
     b = Batch(300, [1] * 129 + [0, 3], 20, torch.float32, seed=9)
