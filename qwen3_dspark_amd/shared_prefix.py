@@ -148,7 +148,7 @@ def shared_capacity(n_req, query_tokens, max_q, n_cu):
     own = width + n_req + slots + (PROMPT_TOKENS // DECODE_TOKENS * slots if prompts else 0)
     tiles = query_tokens // PROMPT_TOKENS + n_req                      # 32-token tiles at most
     return SharedCapacity(n_req + slots - 1, n_req + slots - 1 if prompts else 0, slots, n_req,
-                          max(slots, tiles) if prompts else 0, own + prefix, prefix, prefix + tiles, query_tokens)
+                          max(slots, RESIDENT_PER_CU * n_cu // 8, tiles) if prompts else 0, own + prefix, prefix, prefix + tiles, query_tokens)
 
 
 def mixed_part_ints(c):

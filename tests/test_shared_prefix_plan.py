@@ -154,6 +154,11 @@ def test_large_and_small_plans(n, q, rows, own):
     check_plan([q] * n, [rows + own + q] * n, list(range(n)), groups)
 
 
+def test_columns_where_the_cus_are_no_whole_rounds():
+    """38 CUs per KV head: prompts are cut for 76 workgroups, of which runs take 72."""
+    check_plan([206, 300, 300, 300, 51, 300, 153, 1], [207, 302, 300, 3605, 51, 656, 153, 1], list(range(8)), [], 304)
+
+
 def test_members_that_would_shorten_a_group_stay_out():
     a = ((0, None),)
     lineages = [a, inherited(a, 4000, 1), inherited(a, 4000, 2), inherited(a, 100, 3), inherited(a, 120, 4)]
