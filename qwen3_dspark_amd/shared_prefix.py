@@ -41,6 +41,14 @@ MAX_PREFIX_SEGMENTS = 32
 # prompts of up to 100 tokens over 2,000 rows 27 and 22 us, 3 of 400 over 3,000 65 and 61, 64 requests
 # over 8,192 56 and 57.
 PREFIX_SEGMENT_COST = 400
+# What each further segment costs a group, in keys, and with each of its token tiles: its
+# partials, written and merged.  Without / with it, segments and us a call: 16 requests x 7 tokens
+# over 2,000 rows 8 20.1 / 6 18.4, 12 of 2 groups over 3,056 14 and 17 19.8 / 8 16.3, 4 of 1 token over
+# 10,403 32 39.0 / 15 36.2, 3 prompts of up to 400 over 3,000 3 56.5 / 2 52.7, 64 requests over 8,192
+# the same 3.
+PREFIX_PART_COST = 40, 6
+# More room than PREFIX_TILES does not help prompts: 12 of 2 groups over 6,000 rows in 1, 2
+# and 3 segments 165, 171 and 176 us.
 PREFIX_TILES = 512            # partial tiles that prefix segments may take (more where one segment each needs it)
 TOKEN_INTS = 4
 MAX_BRANCHES = 16             # forks below forks that are looked at for groups of their own
@@ -174,9 +182,10 @@ def prefix_columns(per_cu):
 def prefix_segments(tiles, rows, columns, room):
     """Segments of a group's prefix, for `tiles` token tiles per segment on `columns` workgroup
     slots per KV head: of those that keep MIN_PREFIX_SEGMENT keys each and fit `room`
-    partials, the number whose rounds of slots take the least time."""
+    partials, the number whose rounds of slots and partials take the least time."""
     most = max(1, min(rows // MIN_PREFIX_SEGMENT, MAX_PREFIX_SEGMENTS, room))
-    return min(range(1, most + 1), key=lambda p: -(-tiles * p // columns) * (rows / p + PREFIX_SEGMENT_COST))
+    part = PREFIX_PART_COST[0] + PREFIX_PART_COST[1] * tiles
+    return min(range(1, most + 1), key=lambda p: -(-tiles * p // columns) * (rows / p + PREFIX_SEGMENT_COST) + p * part)
 
 
 def shared_plan(query_lengths, key_lengths, starts, groups, n_cu, capacity, *, xcd_speed=None, slot_balance=True):
