@@ -21,8 +21,8 @@ from collections import namedtuple
 
 import numpy as np
 
-from .schedule import (DECODE_TOKENS, PART_TILE_BYTES, PROMPT_TOKENS, REQ_INTS, RESIDENT_PER_CU, SEGMENT_COST, TILE, WORK_INTS,
-                       XCDS, _balanced_runs, _prompt_columns, prompt_segments, run_count, run_shares)
+from .schedule import (DECODE_TOKENS, MIN_SEGMENT, PART_TILE_BYTES, PROMPT_TOKENS, REQ_INTS, RESIDENT_PER_CU, SEGMENT_COST,
+                       TILE, WORK_INTS, XCDS, _balanced_runs, _prompt_columns, prompt_segments, run_count, run_shares)
 
 PREFIX_TILE = 64              # prefixes end, and are cut, at multiples of this many keys (a ring stage)
 # Fewest key rows that a group must save to be one: sharing takes partials and a second part.
@@ -218,7 +218,9 @@ def shared_plan(query_lengths, key_lengths, starts, groups, n_cu, capacity, *, x
     # the requests' own keys
     decode = [r for r in range(n) if query_lengths[r] <= DECODE_TOKENS]
     prompts = [r for r in range(n) if query_lengths[r] > DECODE_TOKENS]
-    groups_of_runs = min(run_count(sum(own[r] for r in decode) // (2 if prompts else 1), n_cu),
+    # behind a prefix a request may have a few keys: each is worth a run of its own all the
+    # same (by the keys alone 64 requests of 1 token would share 8 runs: 30 us a call)
+    groups_of_runs = min(run_count(sum(max(own[r], MIN_SEGMENT) for r in decode) // (2 if prompts else 1), n_cu),
                          max(XCDS, n_cu // 8 // XCDS * XCDS) if prompts else c.runs)
     per_run = [[] for _ in range(XCDS)]
     if decode:

@@ -154,6 +154,15 @@ def test_large_and_small_plans(n, q, rows, own):
     check_plan([q] * n, [rows + own + q] * n, list(range(n)), groups)
 
 
+def test_requests_with_few_keys_of_their_own_have_runs():
+    """64 requests of one token right behind the prefix: a run each, not 8 a run."""
+    groups = [shared_prefix.Group(list(range(64)), 512, 5)]
+    c = shared_capacity(64, 64, 1, 256)
+    out = shared_plan([1] * 64, [513] * 64, list(range(64)), groups, 256, c).tolist()
+    ranges = out[WORK_INTS * c.run_records:WORK_INTS * c.run_records + c.runs + 1]
+    assert max(b - a for a, b in zip(ranges, ranges[1:])) <= 2 and ranges[-1] <= 80
+
+
 def test_columns_where_the_cus_are_no_whole_rounds():
     """38 CUs per KV head: prompts are cut for 76 workgroups, of which runs take 72."""
     check_plan([206, 300, 300, 300, 51, 300, 153, 1], [207, 302, 300, 3605, 51, 656, 153, 1], list(range(8)), [], 304)
