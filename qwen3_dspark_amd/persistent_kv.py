@@ -631,7 +631,7 @@ class PersistentTargetKV:
             raise ValueError('Varlen cumulative lengths exceed int32')
         groups, shared = (), {}
         if self.shared_prefixes:
-            groups = shared_groups([self._ledger.lineage(i) for i in slots], contexts, slots)
+            groups = shared_groups([self._ledger.lineage(i) for i in slots], contexts, slots, query_lengths)
             shared = dict(groups=groups)
         self.kv_device.build_metadata(self._workspaces[bucket], bucket, slots, contexts, query_lengths, **shared)
         self._transactions += 1

@@ -27,9 +27,15 @@ from .schedule import (DECODE_TOKENS, MIN_SEGMENT, PART_TILE_BYTES, PROMPT_TOKEN
 PREFIX_TILE = 64              # prefixes end, and are cut, at multiples of this many keys (a ring stage)
 # Fewest key rows that a group must save to be one: sharing takes partials and a second part.
 # Shared / each request its own copy, us a call: 2 requests of 7 tokens over 1,000 rows
-# 13.1 / 11.1, 4 over 1,000 14.0 / 12.2, 2 over 4,000 16.3 / 16.7, 16 over 2,000 19.4 / 28.6, 64 over
-# 8,192 56 / 353.
+# 12.2 / 11.4, 4 over 1,000 12.2 / 11.9, 2 over 4,100 15.0 / 17.2, 16 over 2,000 17.5 / 28.6, 64 over 64
+# 14.5 / 12.6, over 128 15.0 / 15.2, over 8,192 56 / 353.
 MIN_SAVED = 4096
+# Groups of more than 32 tokens a request on average are bound by their products, not by
+# reading rows: there the prefix's length decides, whose tiles pay for the partials of so many
+# tokens.  Alike: 2 prompts of 40 over 800 rows 13.5 / 17.4, 2 of 400 over 800 25.2 / 31.0, 8 of 100 over
+# 800 20.5 / 28.2, 16 of 200 over 768 59.7 / 58.6, over 512 53 / 47, over 256 48 / 36, 64 of 40 over
+# 256 42 / 39, 4 of 400 over 800 38.2 / 34.6, over 1,200 44.1 / 43.4, 12 of 220 over 6,000 165 / 234.
+MANY_TOKENS, MIN_LONG_ROWS = 32, 768
 # Prefix workgroups per CU, in the kernel's grid.  Their segments are counted for one: beside
 # them on a CU is a run of the requests' own keys, which memory bounds.  Segments for one / two
 # per CU, us a call: 64 requests of 1 to 8 tokens over 8,192 rows and up to 1,024 own 57 / 61, 8
@@ -83,16 +89,18 @@ def inherited(lineage, rows, origin):
     return (*spans, (origin, None))
 
 
-def shared_groups(lineages, contexts, slots):
+def shared_groups(lineages, contexts, slots, query_lengths=None):
     """[Group(members, rows, slot)] of a batch: the requests of each group hold
-    the same first `rows` rows, a multiple of PREFIX_TILE, which are read from `slot`."""
+    the same first `rows` rows, a multiple of PREFIX_TILE, which are read from `slot`.
+    query_lengths: the requests' tokens (default: few)."""
+    queries = query_lengths or [1] * len(lineages)
     families = {}
     for r, lineage in enumerate(lineages):
         families.setdefault(lineage[0][0], []).append(r)
     groups = []
     for members in families.values():
         if len(members) > 1:
-            groups += _groups_from(lineages, contexts, members, 0, 0)
+            groups += _groups_from(lineages, contexts, queries, members, 0, 0)
     return [Group(sorted(members), rows, slots[min(members)]) for members, rows in groups]
 
 
@@ -100,7 +108,7 @@ def _saved(groups):
     return sum((len(members) - 1) * rows for members, rows in groups)
 
 
-def _groups_from(lineages, contexts, members, depth, branches):
+def _groups_from(lineages, contexts, queries, members, depth, branches):
     """Groups among requests whose lineages are the same up to span `depth`, whose origin they
     have in common too: all of them there, or those of a branch whose lineages stay the
     same for longer apart from the rest, whichever saves more rows."""
@@ -113,28 +121,34 @@ def _groups_from(lineages, contexts, members, depth, branches):
             break
         depth += 1                                             # nobody leaves here
     reach = {r: contexts[r] if lineages[r][depth][1] is None else min(contexts[r], lineages[r][depth][1]) for r in members}
-    chosen, here = [], _groups_at(members, reach)
+    chosen, here = [], _groups_at(members, reach, queries)
     for branch in deeper.values():
         if len(branch) < 2 or branches == MAX_BRANCHES:
             continue
-        apart = _groups_from(lineages, contexts, branch, depth + 1, branches + 1)
+        apart = _groups_from(lineages, contexts, queries, branch, depth + 1, branches + 1)
         inside = {r for group, _ in apart for r in group}
         rest = [r for r in members if r not in inside]
-        without = _groups_at(rest, reach)
+        without = _groups_at(rest, reach, queries)
         if apart and _saved(apart) + _saved(without) > _saved(here):
             members, here = rest, without
             chosen += apart
     return chosen + here
 
 
-def _groups_at(members, reach):
+def _pays(members, rows, queries):
+    if sum(queries[r] for r in members) > MANY_TOKENS * len(members):
+        return rows >= MIN_LONG_ROWS
+    return (len(members) - 1) * rows >= MIN_SAVED
+
+
+def _groups_at(members, reach, queries):
     """[(members, rows)] of requests that have all rows in common up to where each one's reach
     ends: those who would shorten a group more than they gain stay out of it."""
     groups, members = [], sorted(members, key=lambda r: (-reach[r], r))
     while len(members) > 1:
         best = max(range(2, len(members) + 1), key=lambda n: (n - 1) * (reach[members[n - 1]] // PREFIX_TILE))
         rows = reach[members[best - 1]] // PREFIX_TILE * PREFIX_TILE
-        if rows == 0 or (best - 1) * rows < MIN_SAVED:
+        if rows == 0 or not _pays(members[:best], rows, queries):
             break
         groups.append((members[:best], rows))
         members = members[best:]

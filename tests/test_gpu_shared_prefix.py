@@ -16,6 +16,7 @@ DEV = torch.device('cuda:0')
 def groups_of_any_size(monkeypatch):
     from qwen3_dspark_amd import shared_prefix
     monkeypatch.setattr(shared_prefix, 'MIN_SAVED', 0)
+    monkeypatch.setattr(shared_prefix, 'MIN_LONG_ROWS', 0)
 
 
 def build(families, *, layers=1, capacity=6144, rows=512, seed=0, extra=0, shared=True, shuffle=True):

@@ -29,6 +29,7 @@ def test_lineages():
 @pytest.fixture(autouse=True)
 def groups_of_any_size(monkeypatch):
     monkeypatch.setattr(shared_prefix, 'MIN_SAVED', 0)
+    monkeypatch.setattr(shared_prefix, 'MIN_LONG_ROWS', 0)
 
 
 def rows_of(lineage, length):
@@ -213,6 +214,11 @@ def test_groups_that_would_save_little_are_none(monkeypatch):
     assert shared_groups(lineages[:2], [2048] * 2, [0, 1]) == []
     assert [g.length for g in shared_groups(lineages[:3], [2048] * 3, [0, 1, 2])] == [2048]
     assert [g.length for g in shared_groups(lineages, [2048, 1500, 1500, 1500], [0, 1, 2, 3])] == [1472]
+    # prompts: by the rows they share
+    assert [g.length for g in shared_groups(lineages[:2], [2048] * 2, [0, 1], [33, 33])] == [2048]
+    assert [g.length for g in shared_groups(lineages[:2], [800] * 2, [0, 1], [1, 64])] == [768]
+    assert shared_groups(lineages, [767] * 4, [0, 1, 2, 3], [400] * 4) == []
+    assert shared_groups(lineages[:2], [2048] * 2, [0, 1], [32, 32]) == []
 
 
 def test_share_prefix_in_the_store():
